@@ -33,6 +33,12 @@
  *                            modules/windowed_cache/hooks.py:245-290
  *   skv_pack_pages           int4 tier demotion (design.md:130-187; no code in
  *                            the reference)
+ *
+ * Operators without a counterpart in the reference, for the rest of a step:
+ *   skv_rotary               rotary positions of queries and keys
+ *   skv_window_attention     attention with a sliding window and first tokens
+ *                            that stay visible, over plain keys and values
+ *   skv_sample               next token from logits and given random numbers
  */
 #ifndef STICKYKV_B200_H
 #define STICKYKV_B200_H
@@ -140,7 +146,8 @@ const char* skv_last_cuda_error(void);
 /* Bytes of one 8-token int4 page of K and V for head_dim. */
 int32_t skv_page_bytes(int32_t head_dim);
 /* sizeof of the ABI structs (0 skv_layer_desc, 1 skv_evict_plan,
- * 2 skv_evict_args) so a binding can check its own struct layout. */
+ * 2 skv_evict_args, 3 skv_rotary_args, 4 skv_window_args, 5 skv_sample_args)
+ * so a binding can check its own struct layout. */
 int32_t skv_struct_size(int32_t which);
 
 /* Host-only: counts after an eviction (no GPU work). */
@@ -269,6 +276,98 @@ int skv_materialize(const skv_layer_desc* layer, int32_t seq_len, int32_t tier_p
  */
 int skv_pack_pages(const skv_layer_desc* layer, const void* k, const void* v, int32_t first_pos,
                    int32_t n_pages, uint8_t* out, void* stream);
+
+/*
+ * Rotary positions.  With r = rotary_dim and pair i of a head's first r
+ * channels -- (x[i], x[i + r/2]), or (x[2i], x[2i+1]) when interleaved -- at
+ * position p and angle a = p * inv_freq[i] (64-bit product),
+ *   (x1, x2) -> scale * (x1 cos a - x2 sin a, x2 cos a + x1 sin a);
+ * inverse != 0 takes -a (same scale).  Channels r.. are copied.  Arithmetic in
+ * fp32, one rounding to dtype.  Each output may be its own input (same
+ * pointer and strides: in place); otherwise outputs and inputs must not
+ * overlap.  k == NULL: queries only.
+ */
+typedef struct skv_rotary_args {
+  int32_t batch, tokens, num_q_heads, num_kv_heads, head_dim, rotary_dim;
+  int32_t interleaved, inverse, dtype;
+  float scale;
+  const void* q;              /* [batch][heads][tokens][head_dim], unit stride */
+  const void* k;              /* along head_dim, element strides below */
+  void* q_out;
+  void* k_out;
+  int64_t q_stride[3];        /* batch, head, token */
+  int64_t k_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_out_stride[3];
+  const int64_t* positions;   /* [batch][tokens], element strides below (0: shared) */
+  int64_t position_stride[2];
+  const float* inv_freq;      /* [rotary_dim/2] */
+} skv_rotary_args;
+int skv_rotary(const skv_rotary_args* args, void* stream);
+
+/*
+ * Attention with a sliding window and first tokens that stay visible.  Row b's
+ * tokens sit in the slots starts[b] <= j < ends[b] of k/v (NULL: 0 and
+ * k_slots; bounds outside [0, k_slots] are clamped to it); query i sits at
+ * slot p = query_slots[b] + i (NULL: ends[b] - q_tokens + i).  It sees key j
+ * when
+ *   starts <= j <= p < ends and (j - starts < sinks or p - j < window),
+ * out = softmax(scaling * q·k) v over the keys it sees, 0 when it sees none.
+ * Keys and values that a query does not see never reach its output, whatever
+ * they hold.  q/k/v: [batch][heads][tokens or slots][head_dim] in dtype, unit
+ * stride along head_dim, 16-byte aligned base and strides; out
+ * [batch][q_tokens][num_q_heads][head_dim] contiguous.  head_dim 16, 32, 64
+ * or 128.
+ */
+typedef struct skv_window_args {
+  int32_t batch, q_tokens, k_slots, num_q_heads, num_kv_heads, head_dim, dtype;
+  int32_t window;             /* >= 1; the query's own slot counts */
+  int32_t sinks;              /* >= 0 */
+  float scaling;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_stride[3];        /* batch, head, token (elements) */
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  const int32_t* starts;      /* [batch] or NULL */
+  const int32_t* ends;
+  const int32_t* query_slots;
+} skv_window_args;
+size_t skv_window_workspace_size(const skv_window_args* args);
+int skv_window_attention(const skv_window_args* args, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/*
+ * Next token of each row.  With x the row's logits (NaN counts as -inf), m
+ * its largest and w_i = exp((x_i - m) / temperature) in 64 bits, tokens in
+ * descending order of x (equal ones by ascending index):
+ *   top_k > 0   keeps the first top_k;
+ *   top_p < 1   keeps of those the fewest first ones whose mass reaches
+ *               top_p of their mass (always one);
+ *   min_p       keeps of those the ones with w >= min_p;
+ * tokens[b] is the first kept index, in the vocabulary's order, at which the
+ * cumulative kept mass exceeds uniform[b] times the kept mass.  temperature
+ * <= 0 (or NaN): the largest logit, the lowest index among equal ones.  A row
+ * without any logit above -inf gives -1.  Each setting comes from its array
+ * ([batch]) when that is not NULL, else from its scalar.
+ */
+typedef struct skv_sample_args {
+  int32_t batch, vocabulary, dtype;
+  int32_t top_k;
+  float temperature, top_p, min_p;
+  int32_t reserved;
+  const void* logits;         /* [batch][vocabulary], rows row_stride elements apart */
+  int64_t row_stride;
+  const float* uniform;       /* [batch] in [0, 1) */
+  const float* temperatures;  /* [batch] or NULL */
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  int64_t* tokens;            /* [batch] */
+} skv_sample_args;
+int skv_sample(const skv_sample_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -28,6 +28,7 @@ EXPORTS = (
     "skv_evict_workspace_size", "skv_evict", "skv_prefill_workspace_size",
     "skv_prefill_attention", "skv_pack_pages", "skv_decode_attention_noalloc",
     "skv_decode_attention_append", "skv_materialize", "skv_evict_append",
+    "skv_rotary", "skv_window_workspace_size", "skv_window_attention", "skv_sample",
 )
 NOALLOC_SCRATCH_BYTES = 16 << 20
 
@@ -66,6 +67,39 @@ class EvictArgs(C.Structure):
     ]
 
 
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("tokens", C.c_int32), ("num_q_heads", C.c_int32),
+        ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("rotary_dim", C.c_int32),
+        ("interleaved", C.c_int32), ("inverse", C.c_int32), ("dtype", C.c_int32),
+        ("scale", C.c_float), ("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p),
+        ("k_out", C.c_void_p), ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
+        ("q_out_stride", C.c_int64 * 3), ("k_out_stride", C.c_int64 * 3),
+        ("positions", C.c_void_p), ("position_stride", C.c_int64 * 2), ("inv_freq", C.c_void_p),
+    ]
+
+
+class WindowArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("q_tokens", C.c_int32), ("k_slots", C.c_int32),
+        ("num_q_heads", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("dtype", C.c_int32), ("window", C.c_int32), ("sinks", C.c_int32), ("scaling", C.c_float),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("starts", C.c_void_p), ("ends", C.c_void_p), ("query_slots", C.c_void_p),
+    ]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("vocabulary", C.c_int32), ("dtype", C.c_int32), ("top_k", C.c_int32),
+        ("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float),
+        ("reserved", C.c_int32), ("logits", C.c_void_p), ("row_stride", C.c_int64),
+        ("uniform", C.c_void_p), ("temperatures", C.c_void_p), ("top_ks", C.c_void_p),
+        ("top_ps", C.c_void_p), ("min_ps", C.c_void_p), ("tokens", C.c_void_p),
+    ]
+
+
 _lib: Optional[C.CDLL] = None
 _lock = threading.Lock()
 
@@ -95,6 +129,10 @@ def _declare(lib: C.CDLL) -> None:
         "skv_materialize": (C.c_int, [C.POINTER(LayerDesc), I32, I32, P, P, P]),
         "skv_decode_attention_noalloc": (C.c_int, [C.POINTER(LayerDesc), I32, I32, P, I64, I64, P,
                                                    I64, I64, F, P, I32, P]),
+        "skv_rotary": (C.c_int, [C.POINTER(RotaryArgs), P]),
+        "skv_window_workspace_size": (SZ, [C.POINTER(WindowArgs)]),
+        "skv_window_attention": (C.c_int, [C.POINTER(WindowArgs), P, SZ, P]),
+        "skv_sample": (C.c_int, [C.POINTER(SampleArgs), P]),
         "skv_decode_attention_append": (C.c_int, [C.POINTER(LayerDesc), I32, I32, P, P, I64, I64, P,
                                                   I64, I64, P, I64, I64, F, P, I32, P, SZ, P]),
     }
@@ -117,7 +155,7 @@ def lib() -> C.CDLL:
                 _declare(handle)
                 if handle.skv_abi_version() != 1:
                     raise NativeLibraryError("ABI version mismatch")
-                for i, st in enumerate((LayerDesc, EvictPlan, EvictArgs)):
+                for i, st in enumerate((LayerDesc, EvictPlan, EvictArgs, RotaryArgs, WindowArgs, SampleArgs)):
                     if handle.skv_struct_size(i) != C.sizeof(st):
                         raise NativeLibraryError(f"struct layout mismatch for {st.__name__}")
                 _lib = handle

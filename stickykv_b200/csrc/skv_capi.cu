@@ -116,6 +116,9 @@ int32_t skv_struct_size(int32_t which) {
     case 0: return (int32_t)sizeof(skv_layer_desc);
     case 1: return (int32_t)sizeof(skv_evict_plan);
     case 2: return (int32_t)sizeof(skv_evict_args);
+    case 3: return (int32_t)sizeof(skv_rotary_args);
+    case 4: return (int32_t)sizeof(skv_window_args);
+    case 5: return (int32_t)sizeof(skv_sample_args);
   }
   return 0;
 }

@@ -1,0 +1,523 @@
+"""The step operators on the GPU against plain 64-bit forms: rotary positions,
+attention with a sliding window and sinks, token sampling, and a run of them
+together.
+
+Tolerances count roundings.  ``half(dtype)`` is the largest relative error of
+one rounding to the type; a result that is rounded once may be off by that
+much of itself, plus what its 32-bit arithmetic adds (bounded at each test).
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import stickykv_b200 as skv
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U32 = 2.0 ** -24          # half a step of float32
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):          # half the smallest subnormal
+    return torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(shape, dtype, g):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def within(got, want, tol, what=""):
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} outside, worst "
+                           f"{((got.double() - want).abs() / tol).nan_to_num(math.inf).max().item():.3g} of the tolerance")
+
+
+# -- rotary ---------------------------------------------------------------------------------
+
+def rotary_ref(x, pos, inv, inter, scale, inverse):
+    """The rotated tensor in 64 bits and the bound of its 32-bit error: cosine
+    and sine are off by at most 4 ulp of 1 (the angle's rounding to 32 bits, pi
+    * 2^-24, sincospi's 2 ulp and the factor's rounding: under 8 * 2^-24), the
+    two products and their sum by 3 roundings."""
+    r = 2 * inv.numel()
+    a = pos.double().view(*pos.shape[:-1], -1, 1) * inv.double() * (-1 if inverse else 1)
+    a = a.unsqueeze(-3) if a.dim() == 3 else a
+    c, s = a.cos() * scale, a.sin() * scale
+    y = x.double().clone()
+    i = torch.arange(r, device=x.device)
+    i0, i1 = (i[0::2], i[1::2]) if inter else (i[:r // 2], i[r // 2:])
+    x0, x1 = y[..., i0].clone(), y[..., i1].clone()
+    y[..., i0], y[..., i1] = x0 * c - x1 * s, x1 * c + x0 * s
+    e = torch.zeros_like(y)
+    e[..., i0] = e[..., i1] = (x0.abs() + x1.abs()) * abs(scale) * 11 * U32
+    return y, e
+
+
+ROTARY = [  # B, T, Hq, Hkv, D, r, interleaved
+    (1, 1, 1, 1, 2, 2, False), (1, 1, 32, 8, 64, 64, False), (4, 1, 32, 8, 64, 64, True), (2, 7, 3, 1, 128, 128, False),
+    (3, 33, 14, 2, 96, 72, True), (3, 5, 4, 2, 96, 72, False), (1, 257, 2, 2, 80, 40, False), (2, 19, 5, 1, 80, 20, True),
+    (2, 9, 3, 3, 50, 34, False), (2, 9, 3, 3, 50, 2, True), (1, 1000, 8, 8, 32, 32, False),
+]
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("B, T, Hq, Hkv, D, r, inter", ROTARY)
+def test_rotary(B, T, Hq, Hkv, D, r, inter, dt):
+    g = gen(B * T + D)
+    q, k = (normal((B, T, h, D), DT[dt], g).transpose(1, 2) for h in (Hq, Hkv))
+    pos = torch.randint(0, 1 << 20, (B, T), generator=g, device="cuda")
+    inv, _ = skv.rotary_frequencies(r, 500000.0, device="cuda")
+    for inverse, scale in ((False, 1.0), (True, 1.25)):
+        got = skv.apply_rotary(q, k, pos, inv, interleaved=inter, scale=scale, inverse=inverse)
+        for x, y in zip((q, k), got):
+            want, e = rotary_ref(x, pos, inv, inter, scale, inverse)
+            assert y.shape == x.shape and y.stride() == x.stride()
+            within(y, want, e * (1 + half(DT[dt])) + half(DT[dt]) * want.abs() + tiny(DT[dt]), f"{dt} {inverse}")
+            assert torch.equal(y[..., r:], x[..., r:])
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotary_in_place_on_slices_of_one_projection(dt, inter):
+    """Queries and keys as views of one buffer, rotated where they are; the
+    values between them stay."""
+    B, T, Hq, Hkv, D = 2, 21, 6, 2, 64
+    g = gen(5)
+    buf = normal((B, T, Hq + 2 * Hkv, D), DT[dt], g)
+    before = buf.clone()
+    q, k = buf[:, :, :Hq].transpose(1, 2), buf[:, :, Hq:Hq + Hkv].transpose(1, 2)
+    pos = torch.arange(100, 100 + T, device="cuda", dtype=torch.int32)
+    inv, _ = skv.rotary_frequencies(D // 2, device="cuda")
+    apart = skv.apply_rotary(q, k, pos, inv, interleaved=inter)
+    ret = skv.apply_rotary(q, k, pos, inv, interleaved=inter, out=(q, k))
+    assert ret[0] is q and ret[1] is k
+    assert torch.equal(q, apart[0]) and torch.equal(k, apart[1])
+    assert torch.equal(buf[:, :, Hq + Hkv:], before[:, :, Hq + Hkv:])
+
+
+def test_rotary_strides_alignment_and_shapes():
+    g = gen(9)
+    inv, _ = skv.rotary_frequencies(32, device="cuda")
+    pos = torch.tensor([[5, -7, 1 << 30]], device="cuda")
+    wide = normal((2, 4, 3, 67), torch.float16, g)
+    cases = {
+        "odd base": wide[..., 1:33], "odd rows": wide[..., :32], "channels last but one": normal((2, 4, 32, 3), torch.float16, g).transpose(2, 3),
+        "heads expanded": normal((2, 1, 3, 32), torch.float16, g).expand(2, 4, 3, 32), "contiguous": normal((2, 4, 3, 32), torch.float16, g),
+    }
+    for name, q in cases.items():
+        got, none = skv.apply_rotary(q, None, pos, inv)
+        assert none is None
+        want, e = rotary_ref(q, pos, inv, False, 1.0, False)
+        within(got, want, e * 1.01 + half(q.dtype) * want.abs() + tiny(q.dtype), name)
+    for p in (pos[0], pos, pos.expand(2, 3), torch.stack((pos[0],) * 2, -1).t()[:1]):
+        assert torch.equal(skv.apply_rotary(q, None, p, inv)[0], got)
+    empty = torch.empty(0, 4, 3, 32, device="cuda", dtype=torch.float16)
+    assert skv.apply_rotary(empty, empty, pos[0], inv)[0].shape == empty.shape
+    nothing = torch.empty(2, 4, 0, 32, device="cuda", dtype=torch.float16)
+    assert skv.apply_rotary(nothing, nothing, pos[0, :0], inv)[0].shape == nothing.shape
+
+
+def test_rotary_past_32_bit_offsets():
+    """A tensor of over 2^31 elements: the last tokens are the ones checked."""
+    B, H, T, D = 2, 1, (1 << 24) + 37, 64
+    x = torch.empty(B, H, T, D, dtype=torch.bfloat16, device="cuda")
+    x[:, :, -50:] = normal((B, H, 50, D), torch.bfloat16, gen(3))
+    pos = torch.arange(T, device="cuda")
+    inv, _ = skv.rotary_frequencies(D, device="cuda")
+    got, _ = skv.apply_rotary(x, None, pos, inv, out=(x.clone(), None))
+    want, e = rotary_ref(x[:, :, -50:], pos[-50:], inv, False, 1.0, False)
+    within(got[:, :, -50:], want, e * 1.01 + half(x.dtype) * want.abs())
+    del x, got
+    torch.cuda.empty_cache()
+
+
+# -- attention with a window and sinks --------------------------------------------------------
+
+def window_ref(q, k, v, window, sinks, starts=None, ends=None, slots=None, scaling=None):
+    """Output in 64 bits, and per output the sums its error bound is made of:
+    A = sum p |v|, and d, the largest error of a score in 32 bits."""
+    B, Hq, T, D = q.shape
+    Hkv, S = k.shape[1], k.shape[2]
+    scaling = D ** -0.5 if scaling is None else scaling
+    dev = q.device
+    zero = torch.zeros(B, dtype=torch.long, device=dev)
+    st = zero if starts is None else starts.long().clamp(0, S)
+    en = zero + S if ends is None else ends.long().clamp(0, S)
+    first = en - T if slots is None else slots.long()
+    p = (first[:, None] + torch.arange(T, device=dev))[:, :, None]
+    j = torch.arange(S, device=dev)[None, None]
+    st, en = st[:, None, None], en[:, None, None]
+    sees = (j >= st) & (j <= p) & (p < en) & ((j - st < sinks) | (p - j < window))   # [B, T, S]
+    kk = k.double().repeat_interleave(Hq // Hkv, 1)
+    vv = v.double().repeat_interleave(Hq // Hkv, 1)
+    used = sees.any(1)[:, None, :, None]
+    kk, vv = (torch.where(used, x, torch.zeros_like(x)) for x in (kk, vv))
+    a = q.double() @ kk.transpose(2, 3) * scaling
+    a = a.masked_fill(~sees[:, None], -math.inf)
+    pr = torch.softmax(a, -1).nan_to_num(0.0)
+    out, A = pr @ vv, pr @ vv.abs()
+    d = ((q.double().abs() @ kk.abs().transpose(2, 3)) * abs(scaling)).masked_fill(~sees[:, None], 0.0).amax(-1, keepdim=True)
+    n = sees.sum(-1)[:, None, :, None].double()
+    return out.transpose(1, 2), A.transpose(1, 2), d.transpose(1, 2), n.transpose(1, 2)
+
+
+def window_tol(q, ref):
+    """A score is a sum of D products in 32 bits, scaled and moved (D + 6
+    roundings of at most d); the exponent's own error is 2^-21 relative; sums of
+    n weights and products in 32 bits n roundings; weights are rounded once to
+    the 16-bit type before the product with v, and the result once more."""
+    out, A, d, n = ref
+    h = half(q.dtype)
+    t = 2 * ((q.shape[-1] + 6) * U32 * d + 2.0 ** -21) * A + 2 * (n + 4) * U32 * A + h * out.abs()
+    return (t + (h * A if q.dtype != torch.float32 else 0.0)) * (1 + 4 * h) + tiny(q.dtype)
+
+
+def check_window(q, k, v, window, sinks, **kw):
+    got = skv.sink_window_attention(q, k, v, window=window, sinks=sinks, **kw)
+    names = {"query_slots": "slots"}
+    ref = window_ref(q, k, v, k.shape[2] if window is None else window, sinks, **{names.get(a, a): b for a, b in kw.items()})
+    assert got.shape == (q.shape[0], q.shape[2], q.shape[1], q.shape[3]) and got.is_contiguous()
+    within(got, ref[0], window_tol(q, ref), f"{tuple(q.shape)} over {tuple(k.shape)}, window {window}, sinks {sinks}")
+    return got
+
+
+def qkv(B, T, S, Hq, Hkv, D, dt, seed):
+    g = gen(seed)
+    q = normal((B, T, Hq, D), DT[dt], g).transpose(1, 2)
+    return q, normal((B, Hkv, S, D), DT[dt], g), normal((B, Hkv, S, D), DT[dt], g)
+
+
+WINDOW = [  # B, T, S, Hq, Hkv, window, sinks
+    (1, 1, 1, 1, 1, 1, 0), (2, 1, 1, 4, 2, 8, 4), (1, 1, 5, 8, 1, 3, 1), (3, 1, 300, 14, 2, 64, 4), (2, 1, 2000, 32, 8, 700, 5),
+    (1, 1, 4097, 8, 8, 4097, 0), (2, 1, 999, 8, 1, 1, 130), (1, 2, 130, 8, 2, 17, 3), (2, 5, 77, 28, 4, 30, 4), (1, 16, 513, 64, 8, 200, 0),
+    (1, 64, 64, 4, 4, 64, 0), (2, 100, 100, 8, 2, 1, 0), (1, 127, 127, 4, 1, 32, 2), (2, 128, 128, 4, 2, 128, 4), (1, 129, 257, 8, 2, 100, 7),
+    (1, 300, 1111, 8, 2, 257, 130), (2, 385, 385, 14, 2, 129, 4), (1, 700, 700, 32, 8, 90, 200), (3, 260, 260, 3, 3, 1000, 0),
+]
+
+
+@pytest.mark.parametrize("dt, D", [("f32", 16), ("f32", 64), ("f32", 128), ("f16", 16), ("f16", 32), ("f16", 64), ("f16", 128),
+                                   ("bf16", 32), ("bf16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("B, T, S, Hq, Hkv, window, sinks", WINDOW)
+def test_window(B, T, S, Hq, Hkv, window, sinks, dt, D):
+    q, k, v = qkv(B, T, S, Hq, Hkv, D, dt, 7 * T + S)
+    check_window(q, k, v, window, sinks)
+
+
+@pytest.mark.parametrize("dt, D", [("f32", 32), ("f16", 64), ("bf16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("T", [1, 3, 150, 400])
+def test_window_rows_of_unlike_length(dt, D, T):
+    """Left and right padding, rows of no token and of one, queries before and
+    behind their row; what lies in the padding is NaN or infinite and reaches no
+    output, and a query that sees nothing gives zeros."""
+    B, S = 6, 400
+    q, k, v = qkv(B, T, S, 8, 2, D, dt, T)
+    starts = torch.tensor([0, 399, 37, 400, 128, -5], dtype=torch.int32, device="cuda")
+    ends = torch.tensor([400, 400, 300, 400, 129, 1000], dtype=torch.int32, device="cuda")
+    for i, bad in enumerate((math.nan, math.inf, -math.inf, math.nan, math.inf, math.nan)):
+        dead = torch.ones(S, dtype=torch.bool, device="cuda")
+        dead[max(0, int(starts[i])):int(ends[i])] = False
+        k[i, :, dead] = bad
+        v[i, :, dead] = bad
+    for window, sinks in ((20, 4), (None, 0), (129, 140), (1, 1)):
+        for slots in (None, torch.full((B,), S - T, dtype=torch.int32, device="cuda"),
+                      torch.tensor([0, 398, 30, 0, 127, 200], dtype=torch.int32, device="cuda")):
+            got = check_window(q, k, v, window, sinks, starts=starts, ends=ends, query_slots=slots)
+            assert not got[3].any()
+    got = check_window(q, k, v, 20, 4, ends=torch.zeros(B, dtype=torch.int32, device="cuda"))
+    assert not got.any()
+
+
+@pytest.mark.parametrize("dt, D, T", [("f32", 32, 200), ("f16", 64, 200), ("bf16", 128, 333), ("f16", 128, 1), ("bf16", 64, 3)])
+def test_window_unseen_tokens_may_hold_anything(dt, D, T):
+    """Live tokens that some queries see and others do not: one that is not
+    finite reaches exactly the queries that see it."""
+    S, window, sinks = 333, 40, 2
+    q, k, v = qkv(1, T, S, 4, 2, D, dt, 3)
+    at = [S - T, S - 60, S - 1] if T > 60 else [S - 60, S - 50]
+    clean = v.clone()
+    for n, j in enumerate(at):
+        v[:, :, j] = (math.nan, math.inf, -math.inf)[n]
+    got = skv.sink_window_attention(q, k, v, window=window, sinks=sinks)
+    ref = window_ref(q, k, clean, window, sinks)
+    p = torch.arange(S - T, S, device="cuda")
+    hit = torch.zeros(T, dtype=torch.bool, device="cuda")
+    for j in at:
+        hit |= (j <= p) & ((p - j < window) | (j < sinks))
+    assert not got[:, hit].isfinite().any()
+    within(got[:, ~hit], ref[0][:, ~hit], window_tol(q, ref)[:, ~hit])
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("T", [1, 40])
+def test_window_strides(dt, T):
+    """Caches longer than their use, heads and tokens in any order, bases and
+    rows that are not 16-byte aligned, heads shared by expansion."""
+    B, S, Hq, Hkv, D = 2, 200, 6, 2, 64
+    q, k, v = qkv(B, T, S, Hq, Hkv, D, dt, 4)
+    want = check_window(q, k, v, 50, 3)
+    room = torch.full((B, Hkv, S + 57, D), math.nan, dtype=DT[dt], device="cuda")
+    room[:, :, 9:9 + S] = k
+    tokens_first = v.transpose(1, 2).contiguous().transpose(1, 2)
+    odd = torch.empty(B, Hkv, S, D + 1, dtype=DT[dt], device="cuda")[..., 1:]
+    odd.copy_(k)
+    channels = v.transpose(2, 3).contiguous().transpose(2, 3)
+    for kk in (room[:, :, 9:9 + S], odd):
+        for vv in (tokens_first, channels):
+            for qq in (q, q.contiguous(), q.transpose(2, 3).contiguous().transpose(2, 3)):
+                assert torch.equal(skv.sink_window_attention(qq, kk, vv, window=50, sinks=3), want)
+    one = k[:, :1].expand(B, Hkv, S, D)
+    assert torch.equal(skv.sink_window_attention(q, one, one, window=50, sinks=3),
+                       skv.sink_window_attention(q, one.contiguous(), one.contiguous(), window=50, sinks=3))
+    place = torch.empty(B, T, Hq, D, dtype=DT[dt], device="cuda")
+    assert skv.sink_window_attention(q, k, v, window=50, sinks=3, out=place) is place and torch.equal(place, want)
+
+
+def test_window_past_32_bit_offsets():
+    """A cache of over 2^31 elements, most of it never written; decode and a
+    chunk at its far end and, with sinks, at its beginning."""
+    B, Hkv, S, D = 1, 2, (1 << 24) + 1000, 64
+    k, v = (torch.empty(B, Hkv, S, D, dtype=torch.float16, device="cuda") for _ in range(2))
+    g = gen(8)
+    for x in (k, v):
+        x[:, :, -700:] = normal((B, Hkv, 700, D), torch.float16, g)
+        x[:, :, :4] = normal((B, Hkv, 4, D), torch.float16, g)
+    near = [torch.cat((x[:, :, :4], x[:, :, -700:]), 2) for x in (k, v)]
+    for T in (1, 200):
+        q = normal((B, 4, T, D), torch.float16, g)
+        got = skv.sink_window_attention(q, k, v, window=400, sinks=4)
+        ref = window_ref(q, *near, 400, 4)
+        within(got, ref[0], window_tol(q, ref))
+    del k, v
+    torch.cuda.empty_cache()
+
+
+def test_window_large_scores_and_lowest_values():
+    """Scores far apart, and keys of the type's lowest value."""
+    for dt in ("f16", "bf16", "f32"):
+        for T in (1, 200):
+            q, k, v = qkv(1, T, 300, 4, 2, 64, dt, 6)
+            check_window(q, k, v, 70, 4, scaling=4.0)
+            check_window(q, k, v, 70, 4, scaling=-0.5)
+            check_window(q, k, v, 70, 4, scaling=0.0)
+            low = k.clone()
+            low[:, :, ::3] = torch.finfo(DT[dt]).min / 64 if dt == "f16" else -1e4
+            check_window(q, low, v, 70, 4)
+
+
+# -- sampling --------------------------------------------------------------------------------
+
+def sample_ref(x, u, temperature, top_k, top_p, min_p):
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    if not (x > -np.inf).any():
+        return -1
+    order = np.argsort(-x, kind="stable")
+    if not temperature > 0:
+        return int(order[0])
+    if top_k > 0:
+        order = order[:top_k]
+    m = x[order[0]]
+    with np.errstate(invalid="ignore"):
+        w = np.where(x == m, 1.0, np.exp(np.where(x == m, 0.0, x - m) / np.float64(np.float32(temperature))))
+    if top_p < 1:
+        c = np.cumsum(w[order])
+        order = order[:max(1, int(np.searchsorted(c, np.float64(np.float32(top_p)) * c[-1])) + 1)]
+    order = np.sort(order[w[order] >= min(np.float64(np.float32(min_p)), 1.0)])
+    c = np.cumsum(w[order])
+    live = order[w[order] > 0]
+    n = int(np.searchsorted(c, np.float64(np.float32(u)) * c[-1], side="right"))
+    return int(order[n]) if n < len(order) else int(live[-1])
+
+
+def check_sample(x, u, **kw):
+    got = skv.sample_tokens(x, u, **kw)
+    B = x.shape[0]
+    each = [kw[n].cpu().numpy() if torch.is_tensor(kw.get(n)) else np.full(B, kw.get(n, d))
+            for n, d in (("temperature", 1.0), ("top_k", 0), ("top_p", 1.0), ("min_p", 0.0))]
+    want = [sample_ref(r, uu, *s) for r, uu, *s in zip(x.float().cpu().numpy(), u.cpu().numpy(), *each)]
+    assert got.dtype == torch.int64 and got.tolist() == want
+    return got
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("V", [1, 2, 31, 33, 257, 1000, 1023, 4097, 32000, 50001, 128256])
+def test_sample(V, dt):
+    B = 5
+    g = gen(V)
+    for sharp in (0.3, 2.0, 6.0):
+        x = normal((B, V), torch.float32, g).mul(sharp).to(DT[dt])
+        for kw in (dict(), dict(temperature=0.0), dict(temperature=0.7, top_k=50, top_p=0.95), dict(top_k=1), dict(top_k=V),
+                   dict(top_p=0.9), dict(temperature=1.3, top_p=0.5, min_p=0.1), dict(min_p=0.05), dict(top_k=3000, top_p=0.999),
+                   dict(top_p=1e-6), dict(temperature=1e-3), dict(temperature=50.0, top_k=700, min_p=0.9), dict(min_p=1.0)):
+            u = torch.rand(B, generator=g, device="cuda")
+            check_sample(x, u, **kw)
+
+
+def test_sample_settings_of_each_row():
+    B, V = 64, 5003
+    g = gen(2)
+    x = normal((B, V), torch.float32, g) * 3
+    pick = lambda vals, dtype: torch.tensor(vals, dtype=dtype, device="cuda")[  # noqa: E731
+        torch.randint(0, len(vals), (B,), generator=g, device="cuda")]
+    kw = dict(temperature=pick([0.0, -1.0, 0.4, 1.0, 2.0, math.nan], torch.float32), top_k=pick([0, -3, 1, 40, 2000, 99999], torch.int32),
+              top_p=pick([1.0, 2.0, 0.9, 0.3, 0.0, -1.0], torch.float32), min_p=pick([0.0, -1.0, 0.1, 1.0, 3.0], torch.float32))
+    for dt in DT.values():
+        check_sample(x.to(dt), torch.rand(B, generator=g, device="cuda"), **kw)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_sample_ties_and_masks(dt):
+    """Equal logits are taken by index; -inf, NaN, the type's lowest value and
+    +inf; empty rows; both ends of the random numbers."""
+    V = 3001
+    low, inf, nan = torch.finfo(DT[dt]).min, math.inf, math.nan
+    rows = {
+        "all equal": torch.zeros(V), "few levels": (torch.arange(V) * 7 % 3).float(), "one": torch.full((V,), -inf),
+        "all -inf": torch.full((V,), -inf), "all NaN": torch.full((V,), nan), "all lowest": torch.full((V,), low),
+        "lowest and zero": torch.where(torch.arange(V) % 2 == 0, 0.0, low), "NaN between": torch.where(torch.arange(V) % 2 == 0, nan, 1.0),
+        "+inf twice": torch.zeros(V), "signed zeros": torch.where(torch.arange(V) % 3 == 0, -0.0, 0.0),
+    }
+    rows["one"][1234] = -5.0
+    rows["+inf twice"][[17, 2900]] = inf
+    x = torch.stack(list(rows.values())).cuda().to(DT[dt])
+    for u0 in (0.0, 0.25, 0.5, 0.75, 1.0 - 2.0 ** -24):
+        u = torch.full((x.shape[0],), u0, device="cuda")
+        for kw in (dict(), dict(top_k=1), dict(top_k=10), dict(top_p=0.5), dict(top_p=0.9, top_k=1000), dict(min_p=0.5), dict(temperature=0.0),
+                   dict(temperature=0.7, top_p=0.25, top_k=2)):
+            got = check_sample(x, u, **kw)
+            assert got[3] == -1 and got[4] == -1 and got[2] == 1234 and got[8] in (17, 2900)
+
+
+def test_sample_rows_apart_and_odd_bases():
+    g = gen(12)
+    for dt in DT.values():
+        wide = normal((7, 2050), torch.float32, g).to(dt)
+        u = torch.rand(7, generator=g, device="cuda")
+        for x in (wide[:, 1:2001], wide[:, :777], wide[::2, 3:], wide.t().contiguous().t(), wide[:1].expand(7, 2050)):
+            check_sample(x, u[:x.shape[0]].clone(), top_p=0.8)
+            check_sample(x, u[:x.shape[0]].clone(), top_k=33)
+    assert skv.sample_tokens(wide[:0], u[:0]).shape == (0,)
+
+
+def test_sample_frequencies():
+    """4096 evenly spaced random numbers choose each token as often as its
+    probability says, to one draw at each of its two borders."""
+    V, n = 50, 4096
+    x = normal((1, V), torch.float32, gen(1)) * 1.5
+    u = (torch.arange(n, device="cuda") + 0.5) / n
+    got = skv.sample_tokens(x.expand(n, V), u.float(), temperature=0.8, top_k=20)
+    w = torch.softmax(x[0].double() / np.float64(np.float32(0.8)), 0)
+    keep = w >= w.sort(descending=True).values[19]
+    w = torch.where(keep, w, torch.zeros_like(w))
+    count = torch.bincount(got, minlength=V).double()
+    assert ((count - w / w.sum() * n).abs() <= 2).all()
+
+
+# -- streams, graphs and a run together ---------------------------------------------------------
+
+def test_operators_on_another_stream_and_in_graphs_of_their_own():
+    """Called on a side stream; two graphs captured apart and replayed side by
+    side on two streams give what the eager calls give for their inputs."""
+    g = gen(20)
+    inv, _ = skv.rotary_frequencies(64, device="cuda")
+    pos = torch.zeros(2, 1, dtype=torch.long, device="cuda")
+    static = []
+    for i in range(2):
+        q, k, v = qkv(2, 1, 3000, 8, 2, 64, "bf16", 30 + i)
+        static.append(dict(q=q, k=k, v=v, x=normal((2, 9001), torch.float32, g), u=torch.rand(2, generator=g, device="cuda")))
+
+    def step(s):
+        a, _ = skv.apply_rotary(s["q"], None, pos, inv)
+        o = skv.sink_window_attention(a, s["k"], s["v"], window=2500, sinks=4)
+        return o, skv.sample_tokens(s["x"], s["u"], temperature=0.9, top_p=0.9), skv.sample_tokens(s["x"], s["u"], top_k=40)
+
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    for s in static:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(s)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(s))
+        graphs.append(graph)
+    for trial in range(3):
+        for s in static:
+            for name in ("q", "k", "v"):
+                s[name].copy_(normal(s[name].shape, torch.bfloat16, g))
+            s["x"].normal_(generator=g)
+        want = [step(s) for s in static]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for st, graph in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                for _ in range(4):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for w, o in zip(want, outs):
+            assert all(torch.equal(a, b) for a, b in zip(w, o))
+
+
+def test_a_decode_loop_of_all_three():
+    """A tiny one-layer model decodes over a preallocated cache: rotary, append,
+    window attention, logits, sampling.  Each step's attention and token are
+    checked against the 64-bit forms on the step's own inputs, and the loop
+    replayed from one graph gives the same tokens."""
+    B, Hq, Hkv, D, V, S, window, sinks = 3, 8, 2, 64, 501, 64, 10, 2
+    g = gen(77)
+    dtype = torch.bfloat16
+    E = normal((V, Hq * D), dtype, g)
+    Wq, Wk, Wv = (normal((Hq * D, h * D), dtype, g) * 0.05 for h in (Hq, Hkv, Hkv))
+    inv, scale = skv.rotary_frequencies(D // 2, 10000.0, {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32},
+                                        device="cuda")
+    uniforms = torch.rand(40, B, generator=g, device="cuda")
+    k, v = (torch.full((B, Hkv, S, D), math.nan, dtype=dtype, device="cuda") for _ in range(2))
+    tok, n, u = torch.zeros(B, dtype=torch.long, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda"), torch.zeros(B, device="cuda")
+    seen = {}
+
+    def step():
+        h = E[tok]
+        q, kn, vn = ((h @ W).view(B, 1, -1, D).transpose(1, 2) for W in (Wq, Wk, Wv))
+        pos = n.long()[:, None]
+        q, kn = skv.apply_rotary(q, kn, pos, inv, scale=scale)
+        at = pos.view(B, 1, 1, 1).expand(B, Hkv, 1, D)
+        k.scatter_(2, at, kn)
+        v.scatter_(2, at, vn)
+        n.add_(1)
+        o = skv.sink_window_attention(q, k, v, window=window, sinks=sinks, ends=n)
+        logits = (o.reshape(B, -1) @ E.t()) * 0.05
+        seen.update(q=q, o=o, logits=logits)
+        tok.copy_(skv.sample_tokens(logits, u, temperature=0.9, top_k=40, top_p=0.95, min_p=0.01))
+
+    def run(one):
+        tok.zero_(), n.zero_(), k.fill_(math.nan), v.fill_(math.nan)
+        got = []
+        for i in range(40):
+            u.copy_(uniforms[i])
+            one()
+            got.append(tok.tolist())
+        return got
+
+    def checked():
+        step()
+        ref = window_ref(seen["q"], k, v, window, sinks, ends=n)
+        within(seen["o"], ref[0], window_tol(seen["q"], ref))
+        x = seen["logits"].float().cpu().numpy()
+        assert tok.tolist() == [sample_ref(r, uu, 0.9, 40, 0.95, 0.01) for r, uu in zip(x, u.cpu().numpy())]
+
+    with torch.no_grad():
+        want = run(checked)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        assert run(graph.replay) == want
