@@ -335,9 +335,7 @@ typedef struct skv_window_args {
   const int32_t* ends;
   const int32_t* query_slots;
 } skv_window_args;
-size_t skv_window_workspace_size(const skv_window_args* args);
-int skv_window_attention(const skv_window_args* args, void* workspace, size_t workspace_bytes,
-                         void* stream);
+int skv_window_attention(const skv_window_args* args, void* stream);
 
 /*
  * Next token of each row.  With x the row's logits (NaN counts as -inf), m

@@ -28,7 +28,7 @@ EXPORTS = (
     "skv_evict_workspace_size", "skv_evict", "skv_prefill_workspace_size",
     "skv_prefill_attention", "skv_pack_pages", "skv_decode_attention_noalloc",
     "skv_decode_attention_append", "skv_materialize", "skv_evict_append",
-    "skv_rotary", "skv_window_workspace_size", "skv_window_attention", "skv_sample",
+    "skv_rotary", "skv_window_attention", "skv_sample",
 )
 NOALLOC_SCRATCH_BYTES = 16 << 20
 
@@ -130,8 +130,7 @@ def _declare(lib: C.CDLL) -> None:
         "skv_decode_attention_noalloc": (C.c_int, [C.POINTER(LayerDesc), I32, I32, P, I64, I64, P,
                                                    I64, I64, F, P, I32, P]),
         "skv_rotary": (C.c_int, [C.POINTER(RotaryArgs), P]),
-        "skv_window_workspace_size": (SZ, [C.POINTER(WindowArgs)]),
-        "skv_window_attention": (C.c_int, [C.POINTER(WindowArgs), P, SZ, P]),
+        "skv_window_attention": (C.c_int, [C.POINTER(WindowArgs), P]),
         "skv_sample": (C.c_int, [C.POINTER(SampleArgs), P]),
         "skv_decode_attention_append": (C.c_int, [C.POINTER(LayerDesc), I32, I32, P, P, I64, I64, P,
                                                   I64, I64, P, I64, I64, F, P, I32, P, SZ, P]),

@@ -15,6 +15,11 @@ __device__ __forceinline__ __half2 h2(uint32_t x) { return *reinterpret_cast<__h
 template <typename T> struct Op;
 template <> struct Op<__half> {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return u32(__floats2half2_rn(lo, hi)); }
+  static __device__ __forceinline__ void unpack(uint32_t x, float& lo, float& hi) {
+    const float2 f = __half22float2(h2(x));
+    lo = f.x;
+    hi = f.y;
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                              uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -26,6 +31,10 @@ template <> struct Op<__half> {
 };
 template <> struct Op<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return u32(__floats2bfloat162_rn(lo, hi)); }
+  static __device__ __forceinline__ void unpack(uint32_t x, float& lo, float& hi) {
+    lo = __uint_as_float(x << 16);
+    hi = __uint_as_float(x & 0xffff0000u);
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                              uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(

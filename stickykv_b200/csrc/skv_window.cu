@@ -5,56 +5,17 @@
 //   start <= j <= p < end and (j - start < sinks or p - j < window),
 // i.e. the runs [start, min(start + sinks, p + 1)) and
 // [max(start + sinks, p - window + 1, start), p].
-#include "skv_window.cuh"
+#include "skv_window_rows.cuh"
 
 namespace skv {
+int window_few(const WindowParams& p, int dtype, cudaStream_t stream);
 namespace {
 
-// One warp per query, lanes over the channels, online softmax in fp32.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) window_rows_kernel(const WindowParams p) {
-  constexpr int E = D < 32 ? 1 : D / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i = blockIdx.x * 4 + warp, h = blockIdx.y, b = blockIdx.z;
+__global__ void __launch_bounds__(128) window_rows_kernel(const __grid_constant__ WindowParams p) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
   if (i >= p.T) return;
-  const WindowRow row = window_row(p, b);
-  const int pos = row.first + i, kh = h / (p.Hq / p.Hkv);
-  const T* q = (const T*)p.q + b * p.qs[0] + h * p.qs[1] + i * p.qs[2];
-  const T* kb = (const T*)p.k + b * p.ks[0] + kh * p.ks[1];
-  const T* vb = (const T*)p.v + b * p.vs[0] + kh * p.vs[1];
-  float qr[E], acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    qr[e] = lane + 32 * e < D ? ld_f32(q + lane + 32 * e) : 0.f;
-    acc[e] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  auto attend = [&](int j0, int j1) {
-    for (int j = j0; j < j1; ++j) {
-      float dot = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (lane + 32 * e < D) dot += qr[e] * ld_f32(kb + j * p.ks[2] + lane + 32 * e);
-      const float s = warp_sum(dot) * p.scaling;
-      if (s == -INFINITY) continue;  // weighs nothing (and would be -inf - -inf below)
-      const float mn = fmaxf(m, s);
-      const float alpha = expf(m - mn), pr = expf(s - mn);
-      l = l * alpha + pr;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (lane + 32 * e < D) acc[e] = acc[e] * alpha + pr * ld_f32(vb + j * p.vs[2] + lane + 32 * e);
-      m = mn;
-    }
-  };
-  if (pos >= row.start && pos < row.end) {
-    const int sink_end = min(row.sink_end, pos + 1);
-    attend(row.start, sink_end);
-    attend(max(sink_end, pos - p.window + 1), pos + 1);
-  }
-  T* o = (T*)p.out + (((int64_t)b * p.T + i) * p.Hq + h) * D;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (lane + 32 * e < D) st_f32(o + lane + 32 * e, l == 0.f ? 0.f : acc[e] / l);
+  window_one_row<T, D>(p, window_row(p, b), b, h, i, threadIdx.x & 31, 0, D);
 }
 
 template <typename T>
@@ -101,17 +62,9 @@ int check_window(const skv_window_args* a) {
 
 using namespace skv;
 
-extern "C" size_t skv_window_workspace_size(const skv_window_args* a) {
-  if (check_window(a)) return 0;
-  return 0;
-}
-
-extern "C" int skv_window_attention(const skv_window_args* a, void* ws, size_t ws_bytes, void* stream) {
+extern "C" int skv_window_attention(const skv_window_args* a, void* stream) {
   const int rc = check_window(a);
   if (rc) return rc;
-  const size_t need = skv_window_workspace_size(a);
-  if (need && (!ws || ws_bytes < need)) return SKV_ERR_WORKSPACE;
-  if (need && (uintptr_t)ws % 256) return SKV_ERR_MISALIGNED;
   WindowParams p{};
   p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out;
   for (int i = 0; i < 3; ++i) {
@@ -125,9 +78,6 @@ extern "C" int skv_window_attention(const skv_window_args* a, void* ws, size_t w
   p.sinks = a->sinks < a->k_slots ? a->sinks : a->k_slots;
   p.scaling = a->scaling;
   const cudaStream_t s = (cudaStream_t)stream;
-  switch (a->dtype) {
-    case SKV_F32: return launch_rows<float>(p, s);
-    case SKV_F16: return launch_rows<__half>(p, s);
-    default: return launch_rows<__nv_bfloat16>(p, s);
-  }
+  if (a->dtype == SKV_F32) return launch_rows<float>(p, s);
+  return window_few(p, a->dtype, s);
 }

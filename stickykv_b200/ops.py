@@ -4,8 +4,8 @@ visible, and the choice of the next token.
 
 Like the cache they launch on the current stream of the tensors' device, need
 CUDA tensors and the native library (no CPU path), take no part in autograd
-and can be captured into CUDA graphs: scratch memory comes from torch's
-allocator call by call, so graphs that are captured apart share none.
+and can be captured into CUDA graphs (they use no scratch memory, so graphs
+share none).
 """
 
 from __future__ import annotations
@@ -295,13 +295,8 @@ def sink_window_attention(query: Tensor, key: Tensor, value: Tensor, *, window: 
                    _I3(*q.stride()[:3]), _I3(*k.stride()[:3]), _I3(*v.stride()[:3]),
                    None if starts is None else starts.data_ptr(), None if ends is None else ends.data_ptr(),
                    None if query_slots is None else query_slots.data_ptr())
-    L = lib()
-    ref = C.byref(a)
     with _on(q.device):
-        nbytes = L.skv_window_workspace_size(ref)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        check(L.skv_window_attention(ref, None if ws is None else ws.data_ptr(), nbytes, _stream(q.device)),
-              "skv_window_attention")
+        check(lib().skv_window_attention(C.byref(a), _stream(q.device)), "skv_window_attention")
     return out
 
 

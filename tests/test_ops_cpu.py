@@ -167,9 +167,8 @@ def _window_args(**kw):
 ])
 def test_window_c_refusals(kw, status):
     L = _lib.lib()
-    assert L.skv_window_attention(C.byref(_window_args(**kw)), None, 0, None) == status
-    assert L.skv_window_workspace_size(C.byref(_window_args(**kw))) == 0
-    assert L.skv_window_attention(None, None, 0, None) == 1
+    assert L.skv_window_attention(C.byref(_window_args(**kw)), None) == status
+    assert L.skv_window_attention(None, None) == 1
 
 
 @pytest.mark.parametrize("kw, status", [
