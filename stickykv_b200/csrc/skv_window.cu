@@ -9,6 +9,8 @@
 
 namespace skv {
 int window_few(const WindowParams& p, int dtype, cudaStream_t stream);
+bool window_many_supported(const WindowParams& p);
+int window_many(const WindowParams& p, int dtype, cudaStream_t stream);
 namespace {
 
 template <typename T, int D>
@@ -79,5 +81,6 @@ extern "C" int skv_window_attention(const skv_window_args* a, void* stream) {
   p.scaling = a->scaling;
   const cudaStream_t s = (cudaStream_t)stream;
   if (a->dtype == SKV_F32) return launch_rows<float>(p, s);
+  if ((int64_t)p.T * (p.Hq / p.Hkv) > 64 && window_many_supported(p)) return window_many(p, a->dtype, s);
   return window_few(p, a->dtype, s);
 }
