@@ -349,8 +349,10 @@ int skv_window_attention(const skv_window_args* args, void* stream);
  * cumulative kept mass exceeds uniform[b] times the kept mass.  temperature
  * <= 0 (or NaN): the largest logit, the lowest index among equal ones.  A row
  * without any logit above -inf gives -1.  Each setting comes from its array
- * ([batch]) when that is not NULL, else from its scalar.
+ * ([batch]) when that is not NULL, else from its scalar.  vocabulary is at
+ * most SKV_SAMPLE_MAX_VOCABULARY (else SKV_ERR_UNSUPPORTED).
  */
+#define SKV_SAMPLE_MAX_VOCABULARY (1 << 22)
 typedef struct skv_sample_args {
   int32_t batch, vocabulary, dtype;
   int32_t top_k;

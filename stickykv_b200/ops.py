@@ -321,7 +321,7 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
     (float32; int32 for top_k), whose values are not checked: a temperature at
     or below 0 or NaN is greedy, a top_k at or below 0, a top_p from 1 on and
     a min_p at or below 0 cut nothing, a top_p at or below 0 keeps one token.
-    The largest token is always kept."""
+    The largest token is always kept.  V is at most 4,194,304."""
     _same_device("sample_tokens", logits.device, uniform=uniform, out=out)
     _no_grad("sample_tokens", logits, uniform)
     if logits.dim() != 2 or logits.shape[1] == 0:

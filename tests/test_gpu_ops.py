@@ -408,6 +408,20 @@ def test_sample_rows_apart_and_odd_bases():
     assert skv.sample_tokens(wide[:0], u[:0]).shape == (0,)
 
 
+@pytest.mark.parametrize("dt, V", [("f32", 1 << 22), ("f16", 1000003), ("bf16", 400001)])
+def test_sample_large_vocabularies(dt, V):
+    """Rows past what a cluster's shared memory holds, with cuts that keep few
+    and that keep many, and with so many equals that no list holds them."""
+    g = gen(V)
+    x = normal((2, V), torch.float32, g).mul(2.0).to(DT[dt])
+    u = torch.rand(2, generator=g, device="cuda")
+    for kw in (dict(), dict(top_k=100, top_p=0.9), dict(top_k=70000), dict(top_p=0.7), dict(top_k=200000, top_p=0.95, min_p=1e-4)):
+        check_sample(x, u, **kw)
+    few = (torch.arange(V, device="cuda") % 5).to(DT[dt]).expand(2, V)
+    for kw in (dict(top_p=0.8), dict(top_k=V // 2 + 3), dict(top_k=V // 2, top_p=0.93)):
+        check_sample(few, u, **kw)
+
+
 def test_sample_frequencies():
     """4096 evenly spaced random numbers choose each token as often as its
     probability says, to one draw at each of its two borders."""

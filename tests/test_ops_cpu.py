@@ -173,7 +173,8 @@ def test_window_c_refusals(kw, status):
 
 @pytest.mark.parametrize("kw, status", [
     (dict(batch=0), 1), (dict(vocabulary=0), 1), (dict(logits=None), 1), (dict(uniform=None), 1),
-    (dict(tokens=None), 1), (dict(row_stride=-1), 1), (dict(dtype=5), 2), (dict(logits=_P + 1), 3),
+    (dict(tokens=None), 1), (dict(row_stride=-1), 1), (dict(dtype=5), 2), (dict(vocabulary=(1 << 22) + 1), 2),
+    (dict(logits=_P + 1), 3),
     (dict(tokens=_P + 4), 3), (dict(top_ps=_P + 2), 3),
 ])
 def test_sample_c_refusals(kw, status):
