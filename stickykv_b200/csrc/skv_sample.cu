@@ -17,6 +17,8 @@
 // Bound: one row is latency (a handful of cluster barriers), many rows the
 // 64-bit exponentials of a top-p cut (about 16 operations a token at 64 a clock
 // and SM); HBM is read once.
+#include <float.h>
+
 #include "skv_common.cuh"
 
 namespace skv {
@@ -25,7 +27,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBlock = 256;        // tokens a warp takes at once: 8 neighbours a lane
-constexpr int kBins = 2048;
+constexpr int kBins = 1024;
+constexpr int kPerThread = kBins / kThreads;
 constexpr int kList = 2048;        // tokens that are searched in registers, 4 a thread
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kNone = 0x007fffffu;  // key of -inf
@@ -46,15 +49,63 @@ struct SampleParams {
   int staged;    // the row's slice is held in shared memory
 };
 
-// Total order of the values as unsigned integers (NaN and -0 are gone by then).
+// Total order of the values as unsigned integers (without NaN; -0 as +0).
 __device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.f; }
+
+// 16 bytes of logits: NaN to -inf, their maximum and minimum, and as floats.
+template <typename T> struct Pack;
+template <> struct Pack<float> {
+  static constexpr int N = 4;
+  float v[4];
+  __device__ __forceinline__ void clean() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = fmaxf(v[i], -INFINITY);
+  }
+  __device__ __forceinline__ float top() const { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); }
+  __device__ __forceinline__ float least() const { return fminf(fminf(v[0], v[1]), fminf(v[2], v[3])); }
+  __device__ __forceinline__ void floats(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = v[i];
+  }
+};
+template <typename T2> struct Pack2 {
+  static constexpr int N = 8;
+  T2 v[4];
+  __device__ __forceinline__ T2 top2() const { return __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])); }
+  __device__ __forceinline__ T2 least2() const { return __hmin2(__hmin2(v[0], v[1]), __hmin2(v[2], v[3])); }
+};
+template <> struct Pack<__half> : Pack2<__half2> {
+  __device__ __forceinline__ void clean() {
+    const __half2 low = __float2half2_rn(-INFINITY);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __hmax2(v[i], low);
+  }
+  __device__ __forceinline__ float top() const { const float2 f = __half22float2(top2()); return fmaxf(f.x, f.y); }
+  __device__ __forceinline__ float least() const { const float2 f = __half22float2(least2()); return fminf(f.x, f.y); }
+  __device__ __forceinline__ void floats(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float2*>(f)[i] = __half22float2(v[i]);
+  }
+};
+template <> struct Pack<__nv_bfloat16> : Pack2<__nv_bfloat162> {
+  __device__ __forceinline__ void clean() {
+    const __nv_bfloat162 low = __float2bfloat162_rn(-INFINITY);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __hmax2(v[i], low);
+  }
+  __device__ __forceinline__ float top() const { const float2 f = __bfloat1622float2(top2()); return fmaxf(f.x, f.y); }
+  __device__ __forceinline__ float least() const { const float2 f = __bfloat1622float2(least2()); return fminf(f.x, f.y); }
+  __device__ __forceinline__ void floats(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float2*>(f)[i] = __bfloat1622float2(v[i]);
+  }
+};
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 template <typename A>
@@ -74,44 +125,47 @@ __device__ __forceinline__ A peer(const A* p, int rank) {  // another block's co
 
 // What the blocks of a cluster tell one another.
 struct Shared {
-  uint32_t top[1], at[1], least[1];       // largest key, its first index, smallest key above -inf
-  uint32_t warp_min[kWarps];              // of each warp, the smallest of its lanes' largest keys
+  uint64_t warp_best[kWarps];             // of each warp: largest key above the complement of its first block's place
+  uint32_t warp_least[kWarps];            // smallest key
+  uint32_t warp_min[kWarps];              // smallest of its lanes' largest keys
   uint32_t listed[2];
   uint32_t list_lo[2], list_hi[2];        // smallest and largest listed key
-  double mass[2];                         // above the bracket; of all
+  uint32_t finite;                        // smallest key above -inf, where the row holds such
+  uint32_t list_above;                    // tokens above the list
+  double mass[2];                         // above the bracket; below its upper end
   double turn_d[2];                       // bit by bit search, in turns
   uint32_t turn_u[2];
   double kept;                            // mass above the threshold, of the block's tokens
   uint32_t ties;                          // equals of the threshold
   // within the block
-  uint64_t red[kWarps];
-  uint32_t red_u[kWarps];
-  double red_d[kWarps];
+  uint32_t all_min[kWarps * kMaxCluster]; // warp_min of all blocks
+  uint64_t best[kMaxCluster / 2];
+  uint32_t least[kMaxCluster / 2];
+  uint32_t list_end[kMaxCluster];         // listed tokens of the blocks up to each
+  uint64_t red[2][kWarps];                // reductions, in turns
   int found, last;
-  double found_before;
-  uint32_t found_ties;
+  double found_before, carry_mass;
+  uint32_t found_ties, carry_ties;
 };
 
-struct Weight {  // w(x) = 2^((x - m) / T * log2 e) in 64 bits
+// w(x) = 2^((x - m) c), c = log2 e / T, in 64 bits: 2^n 2^f with n whole and
+// |f| <= 1/2, the latter by the polynomial that interpolates 2^f at the 9
+// Chebyshev nodes of [-1/2, 1/2] (off by 1.1e-12 at most; exactly 1 at 0).
+// Where the exponent is above -1000 only; further down a weight counts as none.
+struct Weight {
   double m, c;
   __device__ __forceinline__ double operator()(float x) const {
-    const double y = ((double)x - m) * c;
-    if (x == (float)m) return 1.0;      // also where both are infinite
-    if (!(y > -1000.0)) return x > -INFINITY ? exp2(y) : 0.0;  // near or below the smallest numbers
-    const double t = y + 6755399441055744.0;  // 1.5 * 2^52: rounds to whole numbers
-    const double f = (y - (t - 6755399441055744.0)) * 0.69314718055994530942;
-    // e^f, |f| < 0.35, by its series: the first term left out is below 7e-15
-    double e = 1.0 / 39916800.0;
-    e = fma(e, f, 1.0 / 3628800.0);
-    e = fma(e, f, 1.0 / 362880.0);
-    e = fma(e, f, 1.0 / 40320.0);
-    e = fma(e, f, 1.0 / 5040.0);
-    e = fma(e, f, 1.0 / 720.0);
-    e = fma(e, f, 1.0 / 120.0);
-    e = fma(e, f, 1.0 / 24.0);
-    e = fma(e, f, 1.0 / 6.0);
-    e = fma(e, f, 0.5);
-    e = fma(e, f, 1.0);
+    const double d = (double)x - m;
+    const double t = fma(d, c, 6755399441055744.0);  // 1.5 * 2^52: rounds to whole numbers
+    const double f = fma(d, c, -(t - 6755399441055744.0));
+    double e = 1.3255224878668817e-06;
+    e = fma(e, f, 1.5310079402249296e-05);
+    e = fma(e, f, 0.00015403455852453838);
+    e = fma(e, f, 0.0013333450568000645);
+    e = fma(e, f, 0.009618129159402558);
+    e = fma(e, f, 0.05550410941205933);
+    e = fma(e, f, 0.2402265069581299);
+    e = fma(e, f, 0.6931471805459335);
     e = fma(e, f, 1.0);
     return __hiloint2double(__double2hiint(e) + (__double2loint(t) << 20), __double2loint(e));
   }
@@ -123,32 +177,14 @@ __device__ __forceinline__ A warp_reduce(A v, Op op) {
   for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-template <typename A, typename Op>
-__device__ __forceinline__ A block_reduce(A v, Op op, A* buf) {
-  v = warp_reduce(v, op);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = buf[threadIdx.x & (kWarps - 1)];
-#pragma unroll
-  for (int o = kWarps / 2; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-// inclusive prefix over the block's threads
 template <typename A>
-__device__ __forceinline__ A block_prefix(A v, A* buf) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ A warp_prefix(A v, int n) {  // inclusive, over groups of n lanes
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const A n = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += n;
+  for (int o = 1; o < n; o <<= 1) {
+    const A d = __shfl_up_sync(0xffffffffu, v, o, n);
+    if ((int)(threadIdx.x & (n - 1)) >= o) v += d;
   }
-  __syncthreads();
-  if (lane == 31) buf[warp] = v;
-  __syncthreads();
-  A base = 0;
-  for (int w = 0; w < warp; ++w) base += buf[w];
-  return base + v;
+  return v;
 }
 
 struct Max { template <typename A> __device__ A operator()(A a, A b) const { return a > b ? a : b; } };
@@ -156,14 +192,18 @@ struct Min { template <typename A> __device__ A operator()(A a, A b) const { ret
 struct Sum { template <typename A> __device__ A operator()(A a, A b) const { return a + b; } };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Shared sh;
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t list[kList];
+  // of a search in the list, 8 bits a turn: weights in three parts whose sums over the list fit 32 bits each (one
+  // add of 64 bits is a loop of compare-and-swap, and most listed keys share their upper digits)
+  __shared__ uint32_t digits[4][3][256];
   double* blk_mass = reinterpret_cast<double*>(smem);                       // [per_cta]
   uint32_t* blk_ties = reinterpret_cast<uint32_t*>(blk_mass + p.per_cta);   // [per_cta]
-  T* data = reinterpret_cast<T*>(smem + align_up((size_t)p.per_cta * 12, 16));
+  float* blk_top = reinterpret_cast<float*>(blk_ties + p.per_cta);          // [per_cta] largest logit
+  T* data = reinterpret_cast<T*>(smem + align_up((size_t)p.per_cta * 16, 16));
 
   uint32_t rank, size;
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
@@ -171,332 +211,494 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
   const int C = (int)size, me = (int)rank;
   const int b = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = p.V;
   const T* x = (const T*)p.logits + b * p.stride;
+  const float temp = p.temps ? p.temps[b] : p.temp, share = p.ps ? p.ps[b] : p.p, uniform = p.u[b];
+  const float min_p = p.mins ? p.mins[b] : p.min_p;
+  const int k = p.ks ? p.ks[b] : p.k;
   const int blk0 = me * p.per_cta;                                // first block of this CTA
   const int n_blk = max(0, min(p.per_cta, ceil_div(V, kBlock) - blk0));
-  auto cluster_barrier = [&] {
-    if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-    else __syncthreads();
+  auto cluster_arrive = [&] {
+    if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
   };
-  auto over = [&](const auto* v, auto op) {  // a variable of all blocks of the cluster
+  auto cluster_wait = [&] {
+    if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  };
+  auto cluster_barrier = [&] {
+    if (C > 1) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
+  };
+  // over the block: two buffers in turn, so one barrier each
+  int turn_r = 0;
+  auto block_reduce = [&](auto v, auto op) {
+    using A = decltype(v);
+    A* buf = reinterpret_cast<A*>(sh.red[turn_r++ & 1]);
+    v = warp_reduce(v, op);
+    if (lane == 0) buf[warp] = v;
+    __syncthreads();
+    v = buf[lane & (kWarps - 1)];
+#pragma unroll
+    for (int o = kWarps / 2; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  };
+  auto block_prefix = [&](auto v) {  // inclusive, over the threads
+    using A = decltype(v);
+    A* buf = reinterpret_cast<A*>(sh.red[turn_r++ & 1]);
+    v = warp_prefix(v, 32);
+    if (lane == 31) buf[warp] = v;
+    __syncthreads();
+    const A ends = warp_prefix(buf[lane & (kWarps - 1)], kWarps);
+    const A base = __shfl_sync(0xffffffffu, ends, (warp + kWarps - 1) & (kWarps - 1));
+    return warp ? base + v : v;
+  };
+  auto over = [&](const auto* v, auto op) {  // a variable of all blocks of the cluster, the loads in flight together
     auto r = peer(v, 0);
-    for (int c = 1; c < C; ++c) r = op(r, peer(v, c));
+    decltype(r) e[kMaxCluster];
+#pragma unroll
+    for (int c = 1; c < kMaxCluster; ++c)
+      if (c < C) e[c] = peer(v, c);
+#pragma unroll
+    for (int c = 1; c < kMaxCluster; ++c)
+      if (c < C) r = op(r, e[c]);
     return r;
   };
 
-  // ---- a lane's 8 neighbours of block `blk` (of this CTA) --------------------------------
+  // ---- 8 neighbouring tokens a lane, of block `blk` of this CTA ------------------------------
+  using P = Pack<T>;
+  constexpr int kPacks = 8 / P::N;
   const bool wide = ((uintptr_t)x & 15) == 0;
-  auto fetch = [&](int blk, float (&v)[8]) {  // from global memory
+  auto fetch = [&](int blk, P (&v)[kPacks]) {  // from global memory; -inf behind the row
     const int i0 = (blk0 + blk) * kBlock + lane * 8;
     if (wide && i0 + 8 <= V) {
-      constexpr int N = 16 / sizeof(T);
 #pragma unroll
-      for (int h = 0; h < 8 / N; ++h) {
-        const uint4 w = reinterpret_cast<const uint4*>(x + i0)[h];
-        T e[N];
-        *reinterpret_cast<uint4*>(e) = w;
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[h * N + i] = clean(Elt<T>::to_f32(e[i]));
-      }
+      for (int h = 0; h < kPacks; ++h) *reinterpret_cast<uint4*>(&v[h]) = reinterpret_cast<const uint4*>(x + i0)[h];
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i0 + i < V ? clean(Elt<T>::to_f32(x[i0 + i])) : -INFINITY;
+      for (int h = 0; h < kPacks; ++h) {
+        T e[P::N];
+#pragma unroll
+        for (int i = 0; i < P::N; ++i)
+          e[i] = i0 + h * P::N + i < V ? x[i0 + h * P::N + i] : Elt<T>::from_f32(-INFINITY);
+        *reinterpret_cast<uint4*>(&v[h]) = *reinterpret_cast<uint4*>(e);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < kPacks; ++h) v[h].clean();
+  };
+  bool infinite = false;                       // the largest logit is +inf: such count as 0, the others as -inf
+  auto finite = [&](float v) { return infinite ? (v == INFINITY ? 0.f : -INFINITY) : v; };
+  auto load = [&](int blk, float (&f)[8]) {
+    P v[kPacks];
+    if (p.staged) {
+      const uint4* s = reinterpret_cast<const uint4*>(data + blk * kBlock + lane * 8);
+#pragma unroll
+      for (int h = 0; h < kPacks; ++h) *reinterpret_cast<uint4*>(&v[h]) = s[h];
+    } else {
+      fetch(blk, v);
+    }
+#pragma unroll
+    for (int h = 0; h < kPacks; ++h) v[h].floats(f + h * P::N);
+    if (infinite) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = finite(f[i]);
     }
   };
-  auto load = [&](int blk, float (&v)[8]) {
-    if (!p.staged) return fetch(blk, v);
-    const T* s = data + blk * kBlock + lane * 8;
-    constexpr int N = 16 / sizeof(T);
-#pragma unroll
-    for (int h = 0; h < 8 / N; ++h) {
-      T e[N];
-      *reinterpret_cast<uint4*>(e) = reinterpret_cast<const uint4*>(s)[h];
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[h * N + i] = Elt<T>::to_f32(e[i]);
-    }
-  };
-  auto each = [&](auto&& f) {  // every token of this CTA's slice
+  auto each8 = [&](float least, auto&& f) {    // every 8 tokens of a lane, of this CTA's blocks that reach `least`
     for (int blk = warp; blk < n_blk; blk += kWarps) {
+      if (!(finite(blk_top[blk]) >= least)) continue;
       float v[8];
       load(blk, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f(v[i]);
+      f(blk, v);
     }
   };
 
   // ---- the largest logit --------------------------------------------------------------------
   {
     float mx = -INFINITY, mn = INFINITY;
-    int at = 0;
+    uint64_t best = 0;
     for (int blk = warp; blk < n_blk; blk += kWarps) {
-      float v[8];
+      P v[kPacks];
       fetch(blk, v);
       if (p.staged) {
-        T* s = data + blk * kBlock + lane * 8;
-        constexpr int N = 16 / sizeof(T);
+        uint4* s = reinterpret_cast<uint4*>(data + blk * kBlock + lane * 8);
 #pragma unroll
-        for (int h = 0; h < 8 / N; ++h) {
-          T e[N];
-#pragma unroll
-          for (int i = 0; i < N; ++i) e[i] = Elt<T>::from_f32(v[h * N + i]);
-          reinterpret_cast<uint4*>(s)[h] = *reinterpret_cast<uint4*>(e);
-        }
+        for (int h = 0; h < kPacks; ++h) s[h] = *reinterpret_cast<uint4*>(&v[h]);
       }
+      float hi = v[0].top(), lo = v[0].least();
+      if constexpr (kPacks > 1) hi = fmaxf(hi, v[1].top()), lo = fminf(lo, v[1].least());
+      mx = fmaxf(mx, hi);
+      const int i0 = (blk0 + blk) * kBlock + lane * 8;
+      if (i0 + 8 <= V) {
+        mn = fminf(mn, lo);
+      } else {  // without what fills up the last block
+        float f[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (v[i] > mx) mx = v[i], at = (blk0 + blk) * kBlock + lane * 8 + i;
-        if (v[i] > -INFINITY) mn = fminf(mn, v[i]);
+        for (int h = 0; h < kPacks; ++h) v[h].floats(f + h * P::N);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i0 + i < V) mn = fminf(mn, f[i]);
       }
+      const uint32_t key = __reduce_max_sync(0xffffffffu, key_of(hi));
+      if (lane == 0) blk_top[blk] = value_of(key);
+      if (key > (uint32_t)(best >> 32)) best = (uint64_t)key << 32 | ~(uint32_t)(blk0 + blk);
     }
-    const uint32_t key = key_of(mx);
-    const uint32_t lane_min = warp_reduce(key, Min());
-    const uint32_t top = block_reduce(key, Max(), sh.red_u);
-    const uint32_t first = block_reduce(key == top ? (uint32_t)at : 0xffffffffu, Min(), sh.red_u);
-    const uint32_t least = block_reduce(key_of(mn), Min(), sh.red_u);
-    if (lane == 0) sh.warp_min[warp] = lane_min;
-    if (tid == 0) {
-      sh.top[0] = top;
-      sh.at[0] = first;
-      sh.least[0] = least;
-      sh.listed[0] = sh.listed[1] = 0;
-      sh.list_lo[0] = sh.list_lo[1] = 0xffffffffu;
-      sh.list_hi[0] = sh.list_hi[1] = 0;
-      sh.found = 0x7fffffff;
-      sh.last = -1;
+    const uint32_t lane_min = __reduce_min_sync(0xffffffffu, key_of(mx)), low = __reduce_min_sync(0xffffffffu, key_of(mn));
+    if (lane == 0) {
+      sh.warp_best[warp] = best;
+      sh.warp_least[warp] = low;
+      sh.warp_min[warp] = lane_min;
+    }
+    if (tid < 2) {
+      sh.listed[tid] = 0;
+      sh.list_lo[tid] = 0xffffffffu;
+      sh.list_hi[tid] = 0;
     }
     for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
   }
   cluster_barrier();
-  const uint32_t top = over(&sh.top[0], Max());
-  const float temp = p.temps ? p.temps[b] : p.temp;
-  if (top == kNone || !(temp > 0.f)) {  // nothing above -inf; greedy
-    if (me == 0 && tid == 0) {
-      uint32_t at = 0xffffffffu;
-      for (int c = 0; c < C; ++c)
-        if (peer(&sh.top[0], c) == top) at = min(at, peer(&sh.at[0], c));
-      p.out[b] = top == kNone ? -1 : (int64_t)at;
+  if (tid < kWarps * kMaxCluster) {
+    const bool have = tid < kWarps * C;
+    const int w = tid % kWarps, c = tid / kWarps;
+    uint64_t best = have ? peer(&sh.warp_best[w], c) : 0;
+    uint32_t low = have ? peer(&sh.warp_least[w], c) : 0xffffffffu;
+    sh.all_min[tid] = have ? peer(&sh.warp_min[w], c) : 0;
+    best = warp_reduce(best, Max());
+    low = __reduce_min_sync(0xffffffffu, low);
+    if (lane == 0) {
+      sh.best[warp] = best;
+      sh.least[warp] = low;
     }
-    cluster_barrier();  // no block leaves while others read its variables
+  }
+  __syncthreads();
+  uint64_t best = sh.best[0];
+  uint32_t least_key = sh.least[0];
+#pragma unroll
+  for (int i = 1; i < kMaxCluster / 2; ++i) {
+    best = max(best, sh.best[i]);
+    least_key = min(least_key, sh.least[i]);
+  }
+  uint32_t top = (uint32_t)(best >> 32);
+  if (top == kNone || !(temp > 0.f)) {  // nothing above -inf; greedy
+    cluster_arrive();
+    if (top == kNone) {
+      if (me == 0 && tid == 0) p.out[b] = -1;
+    } else {
+      const int blk = (int)~(uint32_t)best - blk0;  // the first block that reaches it
+      if (blk >= 0 && blk < n_blk && warp == 0) {
+        float v[8];
+        load(blk, v);
+        int at = 8;
+#pragma unroll
+        for (int i = 7; i >= 0; --i)
+          if (key_of(v[i]) == top) at = i;
+        const uint32_t hit = __ballot_sync(0xffffffffu, at < 8);
+        if (lane == __ffs(hit) - 1) p.out[b] = (int64_t)(blk0 + blk) * kBlock + lane * 8 + at;
+      }
+    }
+    cluster_wait();  // no block leaves while others read its variables
     return;
   }
-  const float m = value_of(top), least = value_of(over(&sh.least[0], Min()));
-  const Weight weight{(double)m, 1.4426950408889634074 / (double)temp};
-  auto whole_weight = [&](float v) { return (uint64_t)__double2ll_rn(weight(v) * kUnit); };
+  if (top == 0xff800000u) {
+    infinite = true;
+    top = key_of(0.f);
+    least_key = kNone;
+  }
+  const float m = value_of(top);
+  const double per_t = 1.4426950408889634074 / (double)temp;
+  const Weight weight{(double)m, per_t};
+  // weights of keys below `low_key` count as none
+  const uint32_t low_key = min(top, max(key_of(m - (float)(1000.0 / per_t)), kNone) + 1);
+  auto safe_weight = [&](uint32_t key) { return key >= low_key ? weight(value_of(key)) : 0.0; };
+  auto whole_weight = [&](uint32_t key) { return (uint64_t)__double2ll_rn(safe_weight(key) * kUnit); };
 
   // ---- search over the whole row, bit by bit (counts or masses of keys >= t, those kept) -------
   uint32_t tau = 0, ties = (uint32_t)V;  // kept: keys above tau and `ties` of its equals
   int turn = 0;
   auto count_from = [&](uint32_t t) {
     uint32_t n = 0;
-    each([&](float v) { n += key_of(v) >= t; });
-    n = block_reduce(n, Sum(), sh.red_u);
+    const float least = value_of(t);
+    each8(least, [&](int, const float (&v)[8]) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) n += v[i] >= least;
+    });
+    n = block_reduce(n, Sum());
     if (tid == 0) sh.turn_u[turn & 1] = n;
     cluster_barrier();
     return over(&sh.turn_u[turn++ & 1], Sum());
   };
   auto mass_from = [&](uint32_t t) {
     double s = 0;
-    each([&](float v) {
-      const uint32_t k = key_of(v);
-      if (k >= t && k > tau) s += weight(v);
+    const float least = value_of(max(max(t, tau + 1), low_key));
+    each8(least, [&](int, const float (&v)[8]) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double e = weight(v[i]);
+        if (v[i] >= least) s += e;
+      }
     });
-    s = block_reduce(s, Sum(), sh.red_d);
+    s = block_reduce(s, Sum());
     if (tid == 0) sh.turn_d[turn & 1] = s;
     cluster_barrier();
     s = over(&sh.turn_d[turn++ & 1], Sum());
-    return tau && t <= tau ? s + ties * weight(value_of(tau)) : s;
+    return tau && t <= tau ? s + ties * safe_weight(tau) : s;
   };
   auto slow_mass = [&](float share) {  // tau and ties of the fewest first kept tokens that hold `share` of their mass
     const double goal = (double)share * mass_from(0);
     uint32_t t = 0;
     for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
       if ((t | bit) <= top && mass_from(t | bit) >= goal) t |= bit;
-    const double above = mass_from(t + 1), w = weight(value_of(t));
+    const double above = mass_from(t + 1), w = safe_weight(t);
     uint32_t n = count_from(t) - count_from(t + 1);
     if (t == tau) n = ties;
     const double need = w > 0 ? ceil((goal - above) / w) : 1.0;
     tau = t;
     ties = need >= (double)n ? n : need < 1.0 ? 1u : (uint32_t)need;
   };
+  auto lowest = [&]() -> float {           // the smallest logit above -inf
+    if (least_key == kNone) {
+      float mn = INFINITY;
+      each8(-FLT_MAX, [&](int, const float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (v[i] > -INFINITY) mn = fminf(mn, v[i]);
+      });
+      const uint32_t key = block_reduce(key_of(mn), Min());
+      if (tid == 0) sh.finite = key;
+      cluster_barrier();
+      least_key = over(&sh.finite, Min());
+    }
+    return value_of(least_key);
+  };
 
   // ---- histogram over evenly spaced values below the maximum ------------------------------------
   float per_unit = 0.f;                    // bins per unit of the logit
-  auto bin_of = [&](float v) {             // never falls as v falls
-    const float d = (m - v) * per_unit;
-    return d < (float)(kBins - 1) ? (int)d : kBins - 1;
+  // the distance below the maximum in bins, the last for all further down; rounded to a bin in the low bits of
+  // `place`, and never falls as v falls
+  auto depth = [&](float v) { return fminf((m - v) * per_unit, (float)(kBins - 1)); };
+  auto place = [&](float d) { return d + 8388608.f; };  // 2^23
+  auto bin_at = [&](float t) { return __float_as_uint(t) & (uint32_t)(kBins - 1); };
+  auto spread = [&](float span) {
+    per_unit = span > 0.f ? (float)(kBins - 3) / span : 0.f;
+    if (!(per_unit < INFINITY)) per_unit = 0.f;  // too small a span to divide by
   };
-  // The list of the tokens in bins [lo, hi] (those kept so far), as keys, over all blocks: registers, 4 a thread.
-  uint32_t mine[kList / kThreads];
+  // The list of the tokens from `low` to `high` (those kept so far), as keys,
+  // over all blocks: registers, 4 a thread.  `also` sees every 8 tokens on the
+  // way, but for those of blocks that do not reach `least`.
+  uint32_t mine[kList / kThreads], list_lo = 0, list_hi = 0;
   int lists = 0;                           // lists made so far: each has variables of its own
-  auto collect = [&](int lo, int hi) -> uint32_t {
-    const int z = lists;
+  auto collect = [&](float least, float low, float high, auto&& also, auto&& done) -> uint32_t {
+    const int z = lists++;
     uint32_t lo_k = 0xffffffffu, hi_k = 0;
-    for (int blk = warp; blk < n_blk; blk += kWarps) {
-      float v[8];
-      load(blk, v);
+    for (int i = tid; i < 4 * 3 * 256; i += kThreads) digits[0][0][i] = 0;
+    if (tau) low = fmaxf(low, value_of(tau));
+    each8(least, [&](int, const float (&v)[8]) {
+      also(v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int bin = bin_of(v[i]);
-        const uint32_t k = key_of(v[i]);
-        if (bin >= lo && bin <= hi && k >= tau && k > kNone) {
-          const uint32_t at = atomicAdd(&sh.listed[z], 1u);
-          if (at < kList) list[at] = k;
-          lo_k = min(lo_k, k);
-          hi_k = max(hi_k, k);
+      for (int i = 0; i < 8; ++i)
+        if (v[i] >= low && v[i] <= high && v[i] > -INFINITY) {
+          const uint32_t at = atomicAdd(&sh.listed[z], 1u), key = key_of(v[i]);
+          if (at < kList) list[at] = key;
+          lo_k = min(lo_k, key);
+          hi_k = max(hi_k, key);
         }
-      }
-    }
-    lo_k = warp_reduce(lo_k, Min());
-    hi_k = warp_reduce(hi_k, Max());
+    });
+    lo_k = __reduce_min_sync(0xffffffffu, lo_k);
+    hi_k = __reduce_max_sync(0xffffffffu, hi_k);
     if (lane == 0 && hi_k) {
       atomicMin(&sh.list_lo[z], lo_k);
       atomicMax(&sh.list_hi[z], hi_k);
     }
+    done();
     cluster_barrier();
-    const uint32_t n = over(&sh.listed[z], Sum());
-    ++lists;
+    if (warp == 0) {
+      const uint32_t end = warp_prefix(lane < C ? peer(&sh.listed[z], lane) : 0u, kMaxCluster);
+      if (lane < C) sh.list_end[lane] = end;
+    }
+    list_lo = over(&sh.list_lo[z], Min());
+    list_hi = over(&sh.list_hi[z], Max());
+    __syncthreads();
+    const uint32_t n = sh.list_end[C - 1];
     if (n > kList) return n;
 #pragma unroll
     for (int i = 0; i < kList / kThreads; ++i) {
-      uint32_t at = tid + i * kThreads;
+      const uint32_t at = tid + i * kThreads;
       mine[i] = 0;
       if (at < n) {
         int c = 0;
-        for (uint32_t have; at >= (have = peer(&sh.listed[z], c)); ++c) at -= have;
-        mine[i] = peer(&list[at], c);
+        uint32_t first = 0;
+        for (uint32_t end; at >= (end = sh.list_end[c]); ++c) first = end;
+        mine[i] = peer(&list[at - first], c);
       }
     }
     return n;
   };
-  auto list_lo = [&] { return over(&sh.list_lo[lists - 1], Min()); };
-  auto list_hi = [&] { return over(&sh.list_hi[lists - 1], Max()); };
-  // The largest t with the listed weights of keys >= t at `goal` or more; `extra` counts for t <= tau.
-  auto search = [&](const uint64_t (&w)[kList / kThreads], uint64_t extra, uint64_t goal, uint32_t lo, uint32_t hi) {
-    // the bits that all listed keys share are known
-    const uint32_t differ = lo ^ hi;
-    const int bits = differ ? 32 - __clz(differ) : 0;
-    uint32_t t = bits == 32 ? 0u : hi >> bits << bits;
-    for (int i = bits - 1; i >= 0; --i) {
-      const uint32_t c = t | 1u << i;
-      uint64_t s = 0;
+  // The largest listed key t whose weight together with that of all larger ones
+  // is `goal` or more, 8 bits a turn; `extra` counts as one more of key tau.
+  // Gives the weight above t and that of t and its equals; false: all of them
+  // weigh less than the goal.
+  auto search = [&](const uint64_t (&w)[kList / kThreads], uint64_t extra, uint64_t goal, uint32_t& t, uint64_t& above,
+                    uint64_t& equal) {
+    const uint32_t differ = list_lo ^ list_hi;
+    int bits = differ ? 32 - __clz(differ) : 1;  // the bits above are common to all
+    t = list_hi;
+    above = equal = 0;
+    for (int turn = 0; bits > 0; ++turn) {
+      const int d = min(bits, 8), shift = bits - d;
+      auto add = [&](uint32_t key, uint64_t e) {
+        if (e && (bits == 32 || key >> bits == t >> bits)) {
+          const uint32_t digit = key >> shift & 255u >> (8 - d), low = (uint32_t)e & 0x1fffff, mid = (uint32_t)(e >> 21) & 0x1fffff;
+          if (low) atomicAdd(&digits[turn][0][digit], low);
+          if (mid) atomicAdd(&digits[turn][1][digit], mid);
+          if (e >> 42) atomicAdd(&digits[turn][2][digit], (uint32_t)(e >> 42));
+        }
+      };
 #pragma unroll
       for (int j = 0; j < kList / kThreads; ++j)
-        if (mine[j] >= c) s += w[j];
-      if (block_reduce(s, Sum(), sh.red) + (c <= tau ? extra : 0) >= goal) t = c;
-    }
-    // t's bits below may name a key that no token has: move up to the smallest listed key >= t
-    uint32_t up = 0xffffffffu;
+        if (mine[j]) add(mine[j], w[j]);
+      if (tid == 0) add(tau, extra);
+      __syncthreads();
+      // every warp finds the digit for itself: lane l holds digits 255 - 8 l and the 7 below
+      uint64_t e[8], s = 0;
 #pragma unroll
-    for (int j = 0; j < kList / kThreads; ++j)
-      if (mine[j] >= t) up = min(up, mine[j]);
-    return block_reduce(up, Min(), sh.red_u);
-  };
-  // of the listed keys: (weights above t, equals of t)
-  auto around = [&](const uint64_t (&w)[kList / kThreads], uint32_t t, uint64_t& above, uint32_t& equal) {
-    uint64_t s = 0;
-    uint32_t n = 0;
+      for (int j = 0; j < 8; ++j) {
+        const int digit = 255 - 8 * lane - j;
+        e[j] = digits[turn][0][digit] + ((uint64_t)digits[turn][1][digit] << 21) + ((uint64_t)digits[turn][2][digit] << 42);
+        s += e[j];
+      }
+      uint64_t reached = above + warp_prefix(s, 32);
+      const uint32_t hit = __ballot_sync(0xffffffffu, reached >= goal);
+      if (!hit) return false;
+      const int who = __ffs(hit) - 1;
+      reached -= s;
+      uint32_t digit = 0;
+      uint64_t here = 0;
+      bool done = false;
 #pragma unroll
-    for (int j = 0; j < kList / kThreads; ++j) {
-      if (mine[j] > t) s += w[j];
-      n += mine[j] == t;
+      for (int j = 0; j < 8; ++j) {
+        if (!done) {
+          if (reached + e[j] >= goal) done = true, digit = 255 - 8 * lane - j, here = e[j];
+          else reached += e[j];
+        }
+      }
+      digit = __shfl_sync(0xffffffffu, digit, who);
+      above = __shfl_sync(0xffffffffu, reached, who);
+      equal = __shfl_sync(0xffffffffu, here, who);
+      t = (bits == 32 ? 0u : t >> bits << bits) | digit << shift;
+      bits = shift;
     }
-    above = block_reduce(s, Sum(), sh.red);
-    equal = block_reduce(n, Sum(), sh.red_u);
+    return true;
   };
 
-  const int k = p.ks ? p.ks[b] : p.k;
-  const float share = p.ps ? p.ps[b] : p.p;
   bool have_all = false;                   // the list holds every kept token
   if (k > 0 && k < V) {
     // a value that k tokens reach: that many lanes' largest, of the warps whose lanes do best
     const int warps = C * kWarps, need = ceil_div(k, 32);
-    float low = least;
+    float low = -INFINITY;
     if (need <= warps) {
       // the need-th largest of the warps' smallest lane maxima (equal ones by place)
       uint32_t pick = 0;
-      for (int i = tid; i < warps; i += kThreads) {
-        const uint32_t v = peer(&sh.warp_min[i % kWarps], i / kWarps);
+      if (tid < warps) {
+        const uint32_t v = sh.all_min[tid];
         int before = 0;
         for (int j = 0; j < warps; ++j) {
-          const uint32_t o = peer(&sh.warp_min[j % kWarps], j / kWarps);
-          before += o > v || (o == v && j < i);
+          const uint32_t o = sh.all_min[j];
+          before += o > v || (o == v && j < tid);
         }
         if (before == need - 1) pick = v;
       }
-      pick = block_reduce(pick, Max(), sh.red_u);
-      if (pick > kNone) low = value_of(pick);
+      pick = block_reduce(pick, Max());
+      low = infinite ? finite(value_of(max(pick, kNone))) : value_of(max(pick, kNone));
     }
-    per_unit = m > low ? (float)(kBins - 2) / (m - low) : 0.f;
-    if (!(per_unit < INFINITY)) per_unit = 0.f;   // a span too small or, with +inf, too large to divide
-    each([&](float v) {
-      if (v > -INFINITY) atomicAdd(&hist[bin_of(v)], 1u);
+    if (low == -INFINITY) low = lowest();
+    spread(m - low);
+    if (tid == 0) sh.last = -1;
+    each8(low, [&](int, const float (&v)[8]) {  // the last bin holds all that is further down: not counted
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = depth(v[i]);
+        if (d < (float)(kBins - 2)) atomicAdd(&hist[bin_at(place(d))], 1u);
+      }
     });
     cluster_barrier();
-    // the bin of the k-th largest: four bins a thread, summed over the blocks
-    uint32_t n4[kBins / kThreads], n = 0;
+    // the bin of the k-th largest, summed over the blocks
+    uint32_t count[kPerThread], n = 0;
 #pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) {
-      n4[i] = over(&hist[tid * (kBins / kThreads) + i], Sum());
-      n += n4[i];
+    for (int i = 0; i < kPerThread; ++i) {
+      count[i] = over(&hist[tid * kPerThread + i], Sum());
+      n += count[i];
     }
-    uint32_t before = block_prefix(n, sh.red_u) - n;
-    if (tid == 0) sh.last = -1;
-    __syncthreads();
+    uint32_t before = block_prefix(n) - n;
 #pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) {
-      if (before < (uint32_t)k && before + n4[i] >= (uint32_t)k) {
-        sh.last = tid * (kBins / kThreads) + i;
-        sh.found_ties = before;
+    for (int i = 0; i < kPerThread; ++i) {
+      if (before < (uint32_t)k && before + count[i] >= (uint32_t)k) {
+        sh.last = tid * kPerThread + i;
+        sh.carry_ties = before + count[i];
       }
-      before += n4[i];
+      before += count[i];
     }
     __syncthreads();
     const int bin = sh.last;
-    const uint32_t above = sh.found_ties;
-    if (bin >= 0) {  // fewer than k tokens above -inf: nothing to cut
-      uint32_t rest = (uint32_t)k;
-      const uint32_t in_bin = over(&hist[bin], Sum());
-      have_all = above + in_bin <= kList;
-      if (!have_all) rest -= above;
-      const uint32_t listed = collect(have_all ? 0 : bin, bin);
-      if (listed <= kList) {
-        uint64_t one[kList / kThreads];
+    bool slow = true;
+    if (bin >= 0) {
+      // a little beyond the bin, as its ends are rounded; the counts are checked
+      const float unit = per_unit > 0.f ? 1.f / per_unit : 0.f;
+      const float list_low = m - ((float)bin + 0.75f) * unit, list_high = m - ((float)bin - 0.75f) * unit;
+      have_all = sh.carry_ties <= kList * 3 / 4;
+      uint32_t above_n = 0;
+      const float high = have_all ? INFINITY : list_high;
+      const uint32_t listed = collect(
+          list_low, list_low, high,
+          [&](const float (&v)[8]) {
 #pragma unroll
-        for (int j = 0; j < kList / kThreads; ++j) one[j] = mine[j] != 0;
-        const uint32_t t = search(one, 0, rest, list_lo(), list_hi());
-        uint64_t more;
-        uint32_t equal;
-        around(one, t, more, equal);
-        tau = t;
-        ties = rest - (uint32_t)more;
-      } else if (list_lo() == list_hi()) {
-        tau = list_lo();
-        ties = rest;
-      } else {
-        uint32_t t = 0;
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
-          if (count_from(t | bit) >= (uint32_t)k) t |= bit;
-        ties = (uint32_t)k - count_from(t + 1);
-        tau = t;
+            for (int i = 0; i < 8; ++i) above_n += v[i] > high;
+          },
+          [&] {
+            above_n = block_reduce(above_n, Sum());
+            if (tid == 0) sh.list_above = above_n;
+          });
+      above_n = over(&sh.list_above, Sum());
+      const uint32_t rest = (uint32_t)k - above_n;
+      if (above_n < (uint32_t)k && rest <= listed) {
+        if (listed <= kList) {
+          uint64_t one[kList / kThreads], above, equal;
+#pragma unroll
+          for (int j = 0; j < kList / kThreads; ++j) one[j] = 1;
+          search(one, 0, rest, tau, above, equal);
+          ties = rest - (uint32_t)above;
+          slow = false;
+        } else if (list_lo == list_hi) {
+          tau = list_lo;
+          ties = rest;
+          slow = false;
+        }
       }
+      if (slow) have_all = false;
+    }
+    if (slow && count_from(kNone + 1) > (uint32_t)k) {  // else nothing to cut
+      uint32_t t = 0;
+      for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+        if (count_from(t | bit) >= (uint32_t)k) t |= bit;
+      ties = (uint32_t)k - count_from(t + 1);
+      tau = t;
     }
   }
   if (share < 1.f) {
     uint64_t w[kList / kThreads];
-    auto listed_weights = [&] {  // of the kept ones above tau
+    const uint64_t w_tau = tau ? whole_weight(tau) : 0;
+    auto listed_weights = [&] {            // of the kept ones above tau
 #pragma unroll
-      for (int j = 0; j < kList / kThreads; ++j) w[j] = mine[j] > tau ? whole_weight(value_of(mine[j])) : 0;
+      for (int j = 0; j < kList / kThreads; ++j) w[j] = mine[j] > tau ? whole_weight(mine[j]) : 0;
     };
-    const uint64_t w_tau = tau ? whole_weight(value_of(tau)) : 0;
-    auto cut = [&](uint64_t extra, uint64_t goal) {
-      const uint32_t t = search(w, extra, goal, list_lo(), list_hi());
-      uint64_t above;
-      uint32_t equal;
-      around(w, t, above, equal);
-      const uint64_t wt = whole_weight(value_of(t));
-      if (t == tau) equal = ties;
-      const uint64_t need = wt && goal > above ? (goal - above + wt - 1) / wt : 1;
+    auto cut = [&](uint64_t extra, uint64_t goal) {  // false: the listed ones do not reach the goal
+      uint64_t above, equal;
+      uint32_t t;
+      if (!search(w, extra, goal, t, above, equal)) return false;
+      const uint64_t one = whole_weight(t), need = (goal - above + one - 1) / one, have = equal / one;
       tau = t;
-      ties = need < equal ? (uint32_t)need : equal;
+      ties = (uint32_t)min(need, have);
+      return true;
     };
     if (have_all) {
       listed_weights();
@@ -504,88 +706,88 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
 #pragma unroll
       for (int j = 0; j < kList / kThreads; ++j) s += w[j];
       const uint64_t extra = ties * w_tau;
-      s = block_reduce(s, Sum(), sh.red) + extra;
+      s = block_reduce(s, Sum()) + extra;
+      for (int i = tid; i < 4 * 3 * 256; i += kThreads) digits[0][0][i] = 0;
+      __syncthreads();
       cut(extra, max(1ll, __double2ll_ru((double)share * (double)s)));
     } else {
-      // the bracket from the histogram of weights, each as a share of its bin's largest: 2^-14 of it or less is lost
       if (k > 0 && k < V) {
         cluster_barrier();  // the counts have been read
         for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
         cluster_barrier();
       }
-      const float span = fminf(m - least, 32.f * temp);  // e^-32 * 2^22 tokens weigh nothing against 2^-24
-      per_unit = span > 0.f ? (float)(kBins - 2) / span : 0.f;
-      if (!(per_unit < INFINITY)) per_unit = 0.f;
+      // a histogram of weights, each a whole number of 2^-14 of its bin's middle
+      spread(fminf(m - lowest(), 32.f * temp));  // e^-32 * 2^22 tokens weigh nothing against 2^-24
       const float fall = per_unit > 0.f ? 1.f / (per_unit * temp) : 0.f;  // of the weight's logarithm over a bin
-      each([&](float v) {
-        if (key_of(v) > max(tau, kNone)) {
-          const float d = (m - v) * per_unit;
-          const int bin = d < (float)(kBins - 1) ? (int)d : kBins - 1;
-          const float part = bin < kBins - 1 ? expf(-(d - (float)bin) * fall) : 0.f;
-          atomicAdd(&hist[bin], (uint32_t)(part * 16384.f + 0.5f));
+      if (tid == 0) sh.last = -1;
+      const float kept_from = value_of(max(low_key, tau + 1));
+      each8(kept_from, [&](int, const float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float d = depth(v[i]), t = place(d), off = (t - 8388608.f - d) * fall;
+          // e^off, |off| < 1/60 or so
+          const float part = fmaf(fmaf(off, 0.5f, 1.f), off, 1.f) * 16384.f + 8388608.f;
+          if (d < (float)(kBins - 2) && v[i] >= kept_from) atomicAdd(&hist[bin_at(t)], __float_as_uint(part) & 0x7fffffu);
         }
       });
       cluster_barrier();
-      float s4[kBins / kThreads], s = 0.f;
+      const float fall2 = fall * 1.44269504f;
+      float mass[kPerThread], s = 0.f;
 #pragma unroll
-      for (int i = 0; i < kBins / kThreads; ++i) {
-        const int bin = tid * (kBins / kThreads) + i;
-        float h = 0.f;
-        for (int c = 0; c < C; ++c) h += (float)peer(&hist[bin], c);
-        s4[i] = h * expf(-(float)bin * fall);
-        s += s4[i];
-      }
-      float* red_f = reinterpret_cast<float*>(sh.red_u);
-      float reached = block_prefix(s, red_f) - s;
-      const float all = block_reduce(reached + s, Max(), red_f) + (tau ? (float)ties * (float)weight(value_of(tau)) * 16384.f : 0.f);
-      if (tid == 0) sh.last = -1;
-      __syncthreads();
+      for (int i = 0; i < kPerThread; ++i) {
+        const int bin = tid * kPerThread + i;
+        uint32_t e[kMaxCluster];
+        float h = 0.f;  // the blocks' sums may pass 32 bits together
 #pragma unroll
-      for (int i = 0; i < kBins / kThreads; ++i) {
-        if (reached < share * all) atomicMax(&sh.last, tid * (kBins / kThreads) + i);
-        reached += s4[i];
+        for (int c = 0; c < kMaxCluster; ++c) e[c] = c < C ? peer(&hist[bin], c) : 0;
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) h += (float)e[c];
+        mass[i] = h * exp2f(-(float)bin * fall2);
+        s += mass[i];
+      }
+      float reached = block_prefix(s) - s;
+      const float all = block_reduce(reached + s, Max()) + (tau ? (float)ties * (float)safe_weight(tau) * 16384.f : 0.f);
+#pragma unroll
+      for (int i = 0; i < kPerThread; ++i) {
+        if (reached < share * all && (reached += mass[i]) >= share * all) atomicMax(&sh.last, tid * kPerThread + i);
       }
       __syncthreads();
-      const int bin = max(sh.last, 0), lo = max(0, bin - 1), hi = min(kBins - 1, bin + 1);
-      // exactly: the mass above the bracket, of all kept tokens, and the bracket's tokens
-      double above = 0, total = 0;
-      each([&](float v) {
-        if (key_of(v) > tau) {
-          const double e = weight(v);
-          total += e;
-          if (bin_of(v) < lo) above += e;
-        }
-      });
-      above = block_reduce(above, Sum(), sh.red_d);
-      total = block_reduce(total, Sum(), sh.red_d);
-      if (tid == 0) {
-        sh.mass[0] = above;
-        sh.mass[1] = total;
-      }
-      const uint32_t n = collect(lo, hi);
+      // the bracket: that bin and a neighbour to each side.  Exactly: the mass above it and that of all kept tokens
+      const int bin = max(sh.last, 0);
+      const float unit = per_unit > 0.f ? 1.f / per_unit : 0.f;
+      const float low = m - ((float)bin + 1.5f) * unit, high = m - ((float)bin - 1.5f) * unit;
+      double above = 0, rest = 0;
+      const uint32_t n = collect(
+          kept_from, low, high,
+          [&](const float (&v)[8]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const double e = weight(v[i]);
+              if (v[i] > high) above += e;
+              else if (v[i] >= kept_from) rest += e;
+            }
+          },
+          [&] {
+            above = block_reduce(above, Sum());
+            rest = block_reduce(rest, Sum());
+            if (tid == 0) {
+              sh.mass[0] = above;
+              sh.mass[1] = rest;
+            }
+          });
       above = over(&sh.mass[0], Sum());
-      total = over(&sh.mass[1], Sum());
-      const double extra_d = tau ? ties * weight(value_of(tau)) : 0.0;
-      const double goal = (double)share * (total + extra_d) - above;
+      rest = over(&sh.mass[1], Sum());
+      const float v_tau = tau ? value_of(tau) : -INFINITY;
+      const double goal = (double)share * (above + rest + (tau ? ties * safe_weight(tau) : 0.0)) - above;
+      const bool ends_here = tau && v_tau >= low && v_tau <= high;
       bool found = false;
-      if (n > 0 && n <= kList && goal > 0) {
+      if (goal > 0 && goal < 1024.0 && n > 0 && n <= kList && v_tau <= high) {  // 2^10 * 2^52 and the list's 2^63 fit 64 bits
         listed_weights();
-        uint64_t sum = 0;
-#pragma unroll
-        for (int j = 0; j < kList / kThreads; ++j) sum += w[j];
-        const int tau_bin = tau ? bin_of(value_of(tau)) : kBins;
-        const bool ends_here = tau_bin >= lo && tau_bin <= hi;
-        const uint64_t extra = ends_here ? ties * w_tau : 0;
-        sum = block_reduce(sum, Sum(), sh.red) + extra;
-        const uint64_t g = (uint64_t)max(1ll, __double2ll_ru(goal * kUnit));
-        if (g <= sum && !(ends_here && ties > kList)) {  // more equals would not fit the whole numbers
-          cut(extra, g);
-          found = true;
-        }
-      } else if (n > kList && goal > 0 && list_lo() == list_hi() && list_lo() != tau) {  // equals only
-        const double e = weight(value_of(list_lo())), need = ceil(goal / e);
+        found = cut(ends_here ? ties * w_tau : 0, (uint64_t)max(1ll, __double2ll_ru(goal * kUnit)));
+      } else if (goal > 0 && n > kList && list_lo == list_hi && list_lo > tau && list_lo >= low_key) {  // equals only
+        const double need = ceil(goal / weight(value_of(list_lo)));
         if (need <= (double)n) {
-          tau = list_lo();
+          tau = list_lo;
           ties = (uint32_t)need;
           found = true;
         }
@@ -595,28 +797,39 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
   }
 
   // ---- the draw, in the vocabulary's order --------------------------------------------------------
-  const double floor_w = fminf(p.mins ? p.mins[b] : p.min_p, 1.f);  // the largest always stays
-  // what is surely below the floor is not worth an exponential
-  float floor_v = floor_w > 0 ? m + (float)(log(floor_w) * (double)temp) * 1.0001f - 1e-3f * temp - fabsf(m) * 1e-6f : -INFINITY;
-  if (!(floor_v < INFINITY)) floor_v = -INFINITY;  // of an infinite maximum
+  // kept tokens reach `from`: the smallest key whose weight is min_p or more (the largest always stays)
+  uint32_t from_key = low_key;
+  if (min_p >= 1.f) from_key = top;
+  if (min_p > 0.f && min_p < 1.f) {
+    from_key = key_of((float)((double)m + log((double)min_p) * (double)temp));
+    from_key = min(max(from_key, low_key), top);
+    while (from_key > low_key && weight(value_of(from_key - 1)) >= (double)min_p) --from_key;
+    while (from_key < top && weight(value_of(from_key)) < (double)min_p) ++from_key;
+  }
+  const double w_tau = tau >= from_key ? weight(value_of(tau)) : 0.0;
+  const float from = value_of(max(from_key, tau + 1)), v_tau = value_of(max(tau, kNone));
   double kept = 0;
   uint32_t equal = 0;
   for (int blk = warp; blk < n_blk; blk += kWarps) {
-    float v[8];
-    load(blk, v);
     double s = 0;
     uint32_t n = 0;
+    const float most = finite(blk_top[blk]);
+    if (most >= from || (tau && most >= v_tau)) {
+      float v[8];
+      load(blk, v);
+      double s2[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t kk = key_of(v[i]);
-      n += kk == tau;
-      if (kk > tau && kk > kNone && v[i] >= floor_v) {
+      for (int i = 0; i < 8; ++i) {
         const double e = weight(v[i]);
-        if (e >= floor_w) s += e;
+        if (v[i] >= from) s2[i & 1] += e;
       }
+      if (tau) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n += v[i] == v_tau;
+        n = __reduce_add_sync(0xffffffffu, n);
+      }
+      s = warp_reduce(s2[0] + s2[1], Sum());
     }
-    s = warp_reduce(s, Sum());
-    n = warp_reduce(n, Sum());
     if (lane == 0) {
       blk_mass[blk] = s;
       blk_ties[blk] = n;
@@ -624,8 +837,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
       equal += n;
     }
   }
-  kept = block_reduce(kept, Sum(), sh.red_d);
-  equal = block_reduce(equal, Sum(), sh.red_u);
+  kept = block_reduce(kept, Sum());
+  equal = block_reduce(equal, Sum());
   if (tid == 0) {
     sh.kept = kept;
     sh.ties = equal;
@@ -633,33 +846,35 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     sh.last = -1;
   }
   cluster_barrier();
-  double w_tau = tau ? weight(value_of(tau)) : 0.0;
-  if (!(w_tau >= floor_w)) w_tau = 0.0;
   // the CTA that holds the draw: the first whose cumulative mass exceeds it, else the last with any
   double masses[kMaxCluster], total = 0;
-  uint32_t before_c[kMaxCluster], ties_before = 0;
+  uint32_t equals[kMaxCluster], ties_before = 0;
 #pragma unroll
   for (int c = 0; c < kMaxCluster; ++c) {
-    if (c >= C) break;
-    const uint32_t t = peer(&sh.ties, c), left = ties > ties_before ? ties - ties_before : 0;
-    masses[c] = peer(&sh.kept, c) + (double)min(t, left) * w_tau;
-    before_c[c] = ties_before;
-    total += masses[c];
-    ties_before += t;
+    masses[c] = c < C ? peer(&sh.kept, c) : 0.0;
+    equals[c] = c < C ? peer(&sh.ties, c) : 0;
   }
-  const double goal = (double)p.u[b] * total;
+#pragma unroll
+  for (int c = 0; c < kMaxCluster; ++c) {
+    masses[c] += (double)min(equals[c], ties > ties_before ? ties - ties_before : 0) * w_tau;
+    total += masses[c];
+    ties_before += equals[c];
+  }
+  const double goal = (double)uniform * total;
   double sum = 0, own_before = 0;
   int owner = -1, last_owner = -1;
   uint32_t own_ties = 0;
+  ties_before = 0;
 #pragma unroll
   for (int c = 0; c < kMaxCluster; ++c) {
-    if (c >= C) break;
-    if (c == me) own_before = sum, own_ties = before_c[c];
+    if (c == me) own_before = sum, own_ties = ties_before;
     sum += masses[c];
+    ties_before += equals[c];
     if (masses[c] > 0) last_owner = c;
     if (owner < 0 && sum > goal) owner = c;
   }
   if (owner < 0) owner = last_owner;
+  cluster_arrive();  // done with the others' variables
   if (owner == me) {
     // its 256 tokens, likewise
     double before = own_before;
@@ -667,10 +882,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     for (int base = 0; base < n_blk; base += kThreads) {
       const int i = base + tid;
       const uint32_t t = i < n_blk ? blk_ties[i] : 0;
-      const uint32_t t_inc = block_prefix(t, sh.red_u), t0 = t_before + t_inc - t;
+      const uint32_t t_inc = block_prefix(t), t0 = t_before + t_inc - t;
       const uint32_t left = ties > t0 ? ties - t0 : 0;
       const double mass = i < n_blk ? blk_mass[i] + (double)min(t, left) * w_tau : 0.0;
-      const double inc = before + block_prefix(mass, sh.red_d);
+      const double inc = before + block_prefix(mass);
       if (mass > 0) {
         atomicMax(&sh.last, i);
         if (inc > goal) atomicMin(&sh.found, i);
@@ -682,15 +897,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
         sh.found_before = inc - mass;
         sh.found_ties = t0;
       }
-      // the sums so far, of the last thread
-      if (tid == kThreads - 1) {
-        sh.red[0] = __double_as_longlong(inc);
-        sh.red[1] = t_before + t_inc;
+      if (tid == kThreads - 1) {  // the sums so far
+        sh.carry_mass = inc;
+        sh.carry_ties = t_before + t_inc;
       }
       __syncthreads();
       if (here) break;
-      before = __longlong_as_double(sh.red[0]);
-      t_before = (uint32_t)sh.red[1];
+      before = sh.carry_mass;
+      t_before = sh.carry_ties;
       __syncthreads();
     }
     if (warp == 0) {
@@ -700,29 +914,15 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
       uint32_t n = 0;
       load(blk, v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) n += key_of(v[i]) == tau;
-      uint32_t at = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t d = __shfl_up_sync(0xffffffffu, at, o);
-        if (lane >= o) at += d;
-      }
-      at += sh.found_ties - n;
+      for (int i = 0; i < 8; ++i) n += tau && v[i] == v_tau;
+      uint32_t at = sh.found_ties + warp_prefix(n, 32) - n;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint32_t kk = key_of(v[i]);
-        const bool in = kk > tau || (kk == tau && at++ < ties);
-        e[i] = in ? weight(v[i]) : 0.0;
-        if (!(e[i] >= floor_w)) e[i] = 0.0;
+        e[i] = v[i] >= from ? weight(v[i]) : 0.0;
+        if (tau && v[i] == v_tau && at++ < ties) e[i] = w_tau;
         s += e[i];
       }
-      double inc = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double d = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += d;
-      }
-      inc += sh.found_before;
+      const double inc = sh.found_before + warp_prefix(s, 32);
       const uint32_t any = __ballot_sync(0xffffffffu, s > 0), hit = __ballot_sync(0xffffffffu, s > 0 && inc > goal);
       const int who = hit ? __ffs(hit) - 1 : 31 - __clz(any);
       if (lane == who) {
@@ -740,7 +940,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
       }
     }
   }
-  cluster_barrier();  // no block leaves while others read its variables
+  cluster_wait();  // no block leaves while others read its variables
 }
 
 template <typename T>
@@ -753,12 +953,12 @@ int launch(SampleParams p, int batch, cudaStream_t stream) {
   int c = 1;
   auto bytes = [&](int n) {
     const size_t per = ceil_div(blocks, n);
-    return align_up(per * 12, 16) + per * kBlock * sizeof(T);
+    return per * 16 + per * kBlock * sizeof(T);
   };
   while (c < kMaxCluster && (bytes(c) > (size_t)kMost || (2 * c * kWarps <= 2 * blocks && (int64_t)batch * c * 2 <= 2 * 148))) c *= 2;
   p.per_cta = ceil_div(blocks, c);
   p.staged = bytes(c) <= (size_t)kMost;
-  const size_t smem = p.staged ? bytes(c) : align_up((size_t)p.per_cta * 12, 16);
+  const size_t smem = p.staged ? bytes(c) : (size_t)p.per_cta * 16;
   max_smem_once(done, sample_kernel<T>, kMost);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)batch * c);
