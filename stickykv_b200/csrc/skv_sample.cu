@@ -123,6 +123,14 @@ __device__ __forceinline__ A peer(const A* p, int rank) {  // another block's co
   }
 }
 
+__device__ __forceinline__ uint4 peer4(const uint32_t* p, int rank) {
+  uint32_t a;
+  uint4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
 // What the blocks of a cluster tell one another.
 struct Shared {
   uint64_t warp_best[kWarps];             // of each warp: largest key above the complement of its first block's place
@@ -138,12 +146,15 @@ struct Shared {
   double kept;                            // mass above the threshold, of the block's tokens
   uint32_t ties;                          // equals of the threshold
   // within the block
-  uint32_t all_min[kWarps * kMaxCluster]; // warp_min of all blocks
+  alignas(16) uint32_t all_min[kWarps * kMaxCluster];  // warp_min of all blocks
   uint64_t best[kMaxCluster / 2];
   uint32_t least[kMaxCluster / 2];
   uint32_t list_end[kMaxCluster];         // listed tokens of the blocks up to each
+  uint32_t span_lo, span_hi, all_above;   // of all blocks' lists
   uint64_t red[2][kWarps];                // reductions, in turns
   int found, last;
+  uint32_t pick_key;
+  uint64_t pick_above, pick_equal;
   double found_before, carry_mass;
   uint32_t found_ties, carry_ties;
 };
@@ -195,11 +206,15 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Shared sh;
-  __shared__ uint32_t hist[kBins];
+  __shared__ __align__(16) uint32_t hist[kBins];
+  __shared__ __align__(16) float gathered[2][kBins];  // of half the cluster's blocks each
   __shared__ uint32_t list[kList];
   // of a search in the list, 8 bits a turn: weights in three parts whose sums over the list fit 32 bits each (one
   // add of 64 bits is a loop of compare-and-swap, and most listed keys share their upper digits)
   __shared__ uint32_t digits[4][3][256];
+  // a list of a token a thread: keys and weights
+  __shared__ __align__(16) uint32_t ranked[kThreads];
+  __shared__ __align__(16) unsigned long long ranked_w[kThreads];
   double* blk_mass = reinterpret_cast<double*>(smem);                       // [per_cta]
   uint32_t* blk_ties = reinterpret_cast<uint32_t*>(blk_mass + p.per_cta);   // [per_cta]
   float* blk_top = reinterpret_cast<float*>(blk_ties + p.per_cta);          // [per_cta] largest logit
@@ -284,8 +299,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
         *reinterpret_cast<uint4*>(&v[h]) = *reinterpret_cast<uint4*>(e);
       }
     }
-#pragma unroll
-    for (int h = 0; h < kPacks; ++h) v[h].clean();
   };
   bool infinite = false;                       // the largest logit is +inf: such count as 0, the others as -inf
   auto finite = [&](float v) { return infinite ? (v == INFINITY ? 0.f : -INFINITY) : v; };
@@ -297,6 +310,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       for (int h = 0; h < kPacks; ++h) *reinterpret_cast<uint4*>(&v[h]) = s[h];
     } else {
       fetch(blk, v);
+#pragma unroll
+      for (int h = 0; h < kPacks; ++h) v[h].clean();
     }
 #pragma unroll
     for (int h = 0; h < kPacks; ++h) v[h].floats(f + h * P::N);
@@ -318,9 +333,20 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   {
     float mx = -INFINITY, mn = INFINITY;
     uint64_t best = 0;
-    for (int blk = warp; blk < n_blk; blk += kWarps) {
-      P v[kPacks];
-      fetch(blk, v);
+    constexpr int kAhead = 16 / sizeof(T) / 2;  // blocks whose loads are in flight together
+    P ahead[kAhead][kPacks];
+#pragma unroll 1
+    for (int blk_a = warp; blk_a < n_blk; blk_a += kAhead * kWarps) {
+#pragma unroll
+     for (int a = 0; a < kAhead; ++a)
+      if (blk_a + a * kWarps < n_blk) fetch(blk_a + a * kWarps, ahead[a]);
+#pragma unroll
+     for (int a = 0; a < kAhead; ++a) {
+      const int blk = blk_a + a * kWarps;
+      if (blk >= n_blk) break;
+      P(&v)[kPacks] = ahead[a];
+#pragma unroll
+      for (int h = 0; h < kPacks; ++h) v[h].clean();
       if (p.staged) {
         uint4* s = reinterpret_cast<uint4*>(data + blk * kBlock + lane * 8);
 #pragma unroll
@@ -343,6 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       const uint32_t key = __reduce_max_sync(0xffffffffu, key_of(hi));
       if (lane == 0) blk_top[blk] = value_of(key);
       if (key > (uint32_t)(best >> 32)) best = (uint64_t)key << 32 | ~(uint32_t)(blk0 + blk);
+     }
     }
     const uint32_t lane_min = __reduce_min_sync(0xffffffffu, key_of(mx)), low = __reduce_min_sync(0xffffffffu, key_of(mn));
     if (lane == 0) {
@@ -354,6 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       sh.listed[tid] = 0;
       sh.list_lo[tid] = 0xffffffffu;
       sh.list_hi[tid] = 0;
+      sh.list_above = 0;
     }
     for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
   }
@@ -479,6 +507,24 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   auto depth = [&](float v) { return fminf((m - v) * per_unit, (float)(kBins - 1)); };
   auto place = [&](float d) { return d + 8388608.f; };  // 2^23
   auto bin_at = [&](float t) { return __float_as_uint(t) & (uint32_t)(kBins - 1); };
+  // the cluster's histogram, two bins a thread: 4 bins of every other block a thread, then both halves (as floats: whole
+  // numbers up to 2^24 are exact, larger ones are weights)
+  static_assert(kThreads == 512 && kBins == 1024, "");
+  auto gather = [&](float (&sum)[kPerThread]) {
+    const int g = tid & 255, half = tid >> 8;
+    uint4 e[kMaxCluster / 2];
+#pragma unroll
+    for (int c = 0; c < kMaxCluster / 2; ++c)
+      if (2 * c + half < C) e[c] = peer4(&hist[4 * g], 2 * c + half);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < kMaxCluster / 2; ++c)
+      if (2 * c + half < C) s.x += (float)e[c].x, s.y += (float)e[c].y, s.z += (float)e[c].z, s.w += (float)e[c].w;
+    *reinterpret_cast<float4*>(&gathered[half][4 * g]) = s;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) sum[i] = gathered[0][tid * kPerThread + i] + gathered[1][tid * kPerThread + i];
+  };
   auto spread = [&](float span) {
     per_unit = span > 0.f ? (float)(kBins - 3) / span : 0.f;
     if (!(per_unit < INFINITY)) per_unit = 0.f;  // too small a span to divide by
@@ -486,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   // The list of the tokens from `low` to `high` (those kept so far), as keys,
   // over all blocks: registers, 4 a thread.  `also` sees every 8 tokens on the
   // way, but for those of blocks that do not reach `least`.
-  uint32_t mine[kList / kThreads], list_lo = 0, list_hi = 0;
+  uint32_t mine[kList / kThreads], list_lo = 0, list_hi = 0, listed_n = 0;
   int lists = 0;                           // lists made so far: each has variables of its own
   auto collect = [&](float least, float low, float high, auto&& also, auto&& done) -> uint32_t {
     const int z = lists++;
@@ -495,6 +541,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
     if (tau) low = fmaxf(low, value_of(tau));
     each8(least, [&](int, const float (&v)[8]) {
       also(v);
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) any |= v[i] >= low && v[i] <= high;
+      if (!any) return;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (v[i] >= low && v[i] <= high && v[i] > -INFINITY) {
@@ -512,14 +562,26 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
     }
     done();
     cluster_barrier();
-    if (warp == 0) {
-      const uint32_t end = warp_prefix(lane < C ? peer(&sh.listed[z], lane) : 0u, kMaxCluster);
-      if (lane < C) sh.list_end[lane] = end;
+    if (warp == 0) {  // of each CTA, all in one round: tokens listed, the smallest and the largest, tokens above
+      const int c = lane & 7, what = lane >> 3;
+      const uint32_t* from = what == 0 ? &sh.listed[z] : what == 1 ? &sh.list_lo[z] : what == 2 ? &sh.list_hi[z] : &sh.list_above;
+      const uint32_t got = c < C ? peer(from, c) : what == 1 ? 0xffffffffu : 0;
+      const uint32_t end = warp_prefix(got, 8);  // over the 8 lanes of each kind
+      uint32_t lo = got, hi = got;
+#pragma unroll
+      for (int o = 4; o; o >>= 1) {
+        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      if (what == 0) sh.list_end[c] = end;
+      if (lane == 8) sh.span_lo = lo;
+      if (lane == 16) sh.span_hi = hi;
+      if (lane == 31) sh.all_above = end;
     }
-    list_lo = over(&sh.list_lo[z], Min());
-    list_hi = over(&sh.list_hi[z], Max());
     __syncthreads();
-    const uint32_t n = sh.list_end[C - 1];
+    list_lo = sh.span_lo;
+    list_hi = sh.span_hi;
+    const uint32_t n = sh.list_end[kMaxCluster - 1];
     if (n > kList) return n;
 #pragma unroll
     for (int i = 0; i < kList / kThreads; ++i) {
@@ -532,6 +594,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
         mine[i] = peer(&list[at - first], c);
       }
     }
+    listed_n = n;
+    if (n <= kThreads) {
+      ranked[tid] = mine[0];
+      __syncthreads();
+    }
     return n;
   };
   // The largest listed key t whose weight together with that of all larger ones
@@ -540,6 +607,34 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   // weigh less than the goal.
   auto search = [&](const uint64_t (&w)[kList / kThreads], uint64_t extra, uint64_t goal, uint32_t& t, uint64_t& above,
                     uint64_t& equal) {
+    if (listed_n <= kThreads) {  // each thread looks at all of them for its own
+      ranked_w[tid] = w[0];
+      if (tid == 0) sh.found = 0;
+      __syncthreads();
+      if (mine[0]) {
+        uint64_t more = mine[0] < tau ? extra : 0, same = mine[0] == tau ? extra : 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < listed_n; j += 2) {  // behind the list: key 0, weight 0
+          const uint2 key = *reinterpret_cast<const uint2*>(&ranked[j]);
+          const ulonglong2 e = *reinterpret_cast<const ulonglong2*>(&ranked_w[j]);
+          if (key.x > mine[0]) more += e.x;
+          if (key.y > mine[0]) more += e.y;
+          if (key.x == mine[0]) same += e.x;
+          if (key.y == mine[0]) same += e.y;
+        }
+        if (more < goal && more + same >= goal) {  // its equals find the same
+          sh.found = 1;
+          sh.pick_key = mine[0];
+          sh.pick_above = more;
+          sh.pick_equal = same;
+        }
+      }
+      __syncthreads();
+      t = sh.pick_key;
+      above = sh.pick_above;
+      equal = sh.pick_equal;
+      return sh.found != 0;
+    }
     const uint32_t differ = list_lo ^ list_hi;
     int bits = differ ? 32 - __clz(differ) : 1;  // the bits above are common to all
     t = list_hi;
@@ -602,9 +697,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       if (tid < warps) {
         const uint32_t v = sh.all_min[tid];
         int before = 0;
-        for (int j = 0; j < warps; ++j) {
-          const uint32_t o = sh.all_min[j];
-          before += o > v || (o == v && j < tid);
+#pragma unroll 8
+        for (int j = 0; j < warps; j += 4) {
+          const uint4 o = *reinterpret_cast<const uint4*>(&sh.all_min[j]);
+          before += (o.x > v || (o.x == v && j < tid)) + (o.y > v || (o.y == v && j + 1 < tid)) +
+                    (o.z > v || (o.z == v && j + 2 < tid)) + (o.w > v || (o.w == v && j + 3 < tid));
         }
         if (before == need - 1) pick = v;
       }
@@ -623,10 +720,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
     });
     cluster_barrier();
     // the bin of the k-th largest, summed over the blocks
-    uint32_t count[kPerThread], n = 0;
+    float sums[kPerThread];
+    gather(sums);
+    uint32_t count[kPerThread], n = 0;  // 2^22 tokens at most: exact
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      count[i] = over(&hist[tid * kPerThread + i], Sum());
+      count[i] = (uint32_t)sums[i];
       n += count[i];
     }
     uint32_t before = block_prefix(n) - n;
@@ -658,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
             above_n = block_reduce(above_n, Sum());
             if (tid == 0) sh.list_above = above_n;
           });
-      above_n = over(&sh.list_above, Sum());
+      above_n = sh.all_above;
       const uint32_t rest = (uint32_t)k - above_n;
       if (above_n < (uint32_t)k && rest <= listed) {
         if (listed <= kList) {
@@ -733,16 +832,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       cluster_barrier();
       const float fall2 = fall * 1.44269504f;
       float mass[kPerThread], s = 0.f;
+      gather(mass);
 #pragma unroll
       for (int i = 0; i < kPerThread; ++i) {
-        const int bin = tid * kPerThread + i;
-        uint32_t e[kMaxCluster];
-        float h = 0.f;  // the blocks' sums may pass 32 bits together
-#pragma unroll
-        for (int c = 0; c < kMaxCluster; ++c) e[c] = c < C ? peer(&hist[bin], c) : 0;
-#pragma unroll
-        for (int c = 0; c < kMaxCluster; ++c) h += (float)e[c];
-        mass[i] = h * exp2f(-(float)bin * fall2);
+        mass[i] *= exp2f(-(float)(tid * kPerThread + i) * fall2);
         s += mass[i];
       }
       float reached = block_prefix(s) - s;
@@ -756,20 +849,24 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       const int bin = max(sh.last, 0);
       const float unit = per_unit > 0.f ? 1.f / per_unit : 0.f;
       const float low = m - ((float)bin + 1.5f) * unit, high = m - ((float)bin - 1.5f) * unit;
-      double above = 0, rest = 0;
+      double above = 0, rest = 0, above2 = 0, rest2 = 0;
       const uint32_t n = collect(
           kept_from, low, high,
           [&](const float (&v)[8]) {
+            double e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const double e = weight(v[i]);
-              if (v[i] > high) above += e;
-              else if (v[i] >= kept_from) rest += e;
+            for (int i = 0; i < 8; ++i) e[i] = weight(v[i]);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+              if (v[i] > high) above += e[i];
+              if (v[i + 1] > high) above2 += e[i + 1];
+              if (v[i] <= high && v[i] >= kept_from) rest += e[i];
+              if (v[i + 1] <= high && v[i + 1] >= kept_from) rest2 += e[i + 1];
             }
           },
           [&] {
-            above = block_reduce(above, Sum());
-            rest = block_reduce(rest, Sum());
+            above = block_reduce(above + above2, Sum());
+            rest = block_reduce(rest + rest2, Sum());
             if (tid == 0) {
               sh.mass[0] = above;
               sh.mass[1] = rest;
