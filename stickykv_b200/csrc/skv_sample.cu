@@ -136,8 +136,8 @@ struct Shared {
   uint64_t warp_best[kWarps];             // of each warp: largest key above the complement of its first block's place
   uint32_t warp_least[kWarps];            // smallest key
   uint32_t warp_min[kWarps];              // smallest of its lanes' largest keys
-  uint32_t listed[2];
-  uint32_t list_lo[2], list_hi[2];        // smallest and largest listed key
+  uint32_t listed[3];
+  uint32_t list_lo[3], list_hi[3];        // smallest and largest listed key
   uint32_t finite;                        // smallest key above -inf, where the row holds such
   uint32_t list_above;                    // tokens above the list
   double mass[2];                         // above the bracket; below its upper end
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       sh.warp_least[warp] = low;
       sh.warp_min[warp] = lane_min;
     }
-    if (tid < 2) {
+    if (tid < 3) {
       sh.listed[tid] = 0;
       sh.list_lo[tid] = 0xffffffffu;
       sh.list_hi[tid] = 0;
@@ -538,18 +538,20 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
     const int z = lists++;
     uint32_t lo_k = 0xffffffffu, hi_k = 0;
     for (int i = tid; i < 4 * 3 * 256; i += kThreads) digits[0][0][i] = 0;
-    if (tau) low = fmaxf(low, value_of(tau));
+    low = fmaxf(low, tau ? value_of(tau) : -FLT_MAX);
     each8(least, [&](int, const float (&v)[8]) {
       also(v);
-      bool any = false;
+      uint32_t n = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) any |= v[i] >= low && v[i] <= high;
-      if (!any) return;
+      for (int i = 0; i < 8; ++i) n += v[i] >= low && v[i] <= high;
+      if (n == 0) return;
+      uint32_t at = atomicAdd(&sh.listed[z], n);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (v[i] >= low && v[i] <= high && v[i] > -INFINITY) {
-          const uint32_t at = atomicAdd(&sh.listed[z], 1u), key = key_of(v[i]);
+        if (v[i] >= low && v[i] <= high) {
+          const uint32_t key = key_of(v[i]);
           if (at < kList) list[at] = key;
+          ++at;
           lo_k = min(lo_k, key);
           hi_k = max(hi_k, key);
         }
@@ -687,7 +689,26 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   };
 
   bool have_all = false;                   // the list holds every kept token
-  if (k > 0 && k < V) {
+  const int n_all = ceil_div(V, kBlock);
+  if (k > 0 && 2 * k <= min(kThreads, n_all)) {
+    // few: a value that k of the row's groups of tokens reach, by the upper 20 bits of its key; all tokens from there on
+    // are little more than k
+    uint32_t best_of = 0, t = 0;
+    for (int i = tid; i < n_all; i += kThreads) best_of = max(best_of, key_of(finite(peer(&blk_top[i % p.per_cta], i / p.per_cta))));
+    for (uint32_t bit = 0x80000000u; bit > 0x800u; bit >>= 1)
+      if (__syncthreads_count(best_of >= (t | bit)) >= k) t |= bit;
+    const float low = value_of(max(t, kNone + 1));
+    const uint32_t listed = collect(low, low, INFINITY, [](const float (&)[8]) {}, [] {});
+    if (listed >= (uint32_t)k && listed <= kList) {
+      uint64_t one[kList / kThreads], above, equal;
+#pragma unroll
+      for (int j = 0; j < kList / kThreads; ++j) one[j] = mine[j] != 0;
+      search(one, 0, (uint32_t)k, tau, above, equal);
+      ties = (uint32_t)k - (uint32_t)above;
+      have_all = true;
+    }
+  }
+  if (k > 0 && k < V && !have_all) {
     // a value that k tokens reach: that many lanes' largest, of the warps whose lanes do best
     const int warps = C * kWarps, need = ceil_div(k, 32);
     float low = -INFINITY;
@@ -763,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
         if (listed <= kList) {
           uint64_t one[kList / kThreads], above, equal;
 #pragma unroll
-          for (int j = 0; j < kList / kThreads; ++j) one[j] = 1;
+          for (int j = 0; j < kList / kThreads; ++j) one[j] = mine[j] != 0;
           search(one, 0, rest, tau, above, equal);
           ties = rest - (uint32_t)above;
           slow = false;
@@ -816,7 +837,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
         cluster_barrier();
       }
       // a histogram of weights, each a whole number of 2^-14 of its bin's middle
-      spread(fminf(m - lowest(), 32.f * temp));  // e^-32 * 2^22 tokens weigh nothing against 2^-24
+      // as deep as what is further down, all V tokens of it, weighs a thousandth of what the cut leaves out
+      spread(fminf(m - lowest(), temp * (logf((float)V / fmaxf(1.f - share, 1e-7f)) + 7.f)));
       const float fall = per_unit > 0.f ? 1.f / (per_unit * temp) : 0.f;  // of the weight's logarithm over a bin
       if (tid == 0) sh.last = -1;
       const float kept_from = value_of(max(low_key, tau + 1));
@@ -845,10 +867,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
         if (reached < share * all && (reached += mass[i]) >= share * all) atomicMax(&sh.last, tid * kPerThread + i);
       }
       __syncthreads();
-      // the bracket: that bin and a neighbour to each side.  Exactly: the mass above it and that of all kept tokens
+      // the bracket: that bin and a little beyond.  Exactly: the mass above it and that of all kept tokens
       const int bin = max(sh.last, 0);
       const float unit = per_unit > 0.f ? 1.f / per_unit : 0.f;
-      const float low = m - ((float)bin + 1.5f) * unit, high = m - ((float)bin - 1.5f) * unit;
+      const float low = m - ((float)bin + 0.65f) * unit, high = m - ((float)bin - 0.65f) * unit;
       double above = 0, rest = 0, above2 = 0, rest2 = 0;
       const uint32_t n = collect(
           kept_from, low, high,
@@ -1052,7 +1074,7 @@ int launch(SampleParams p, int batch, cudaStream_t stream) {
     const size_t per = ceil_div(blocks, n);
     return per * 16 + per * kBlock * sizeof(T);
   };
-  while (c < kMaxCluster && (bytes(c) > (size_t)kMost || (2 * c * kWarps <= 2 * blocks && (int64_t)batch * c * 2 <= 2 * 148))) c *= 2;
+  while (c < kMaxCluster && (bytes(c) > (size_t)kMost || (c * kWarps <= blocks && (int64_t)batch * c * 2 <= 148))) c *= 2;
   p.per_cta = ceil_div(blocks, c);
   p.staged = bytes(c) <= (size_t)kMost;
   const size_t smem = p.staged ? bytes(c) : (size_t)p.per_cta * 16;
