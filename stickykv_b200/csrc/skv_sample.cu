@@ -30,6 +30,8 @@ constexpr int kBlock = 256;        // tokens a warp takes at once: 8 neighbours 
 constexpr int kBins = 1024;
 constexpr int kPerThread = kBins / kThreads;
 constexpr int kList = 2048;        // tokens that are searched in registers, 4 a thread
+constexpr int kRanked = 192;       // listed tokens up to here are compared each with each (n^2 / 512 steps a thread; more take
+                                   // three to four turns of 8 bits, about 1.5 us each)
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kNone = 0x007fffffu;  // key of -inf
 constexpr double kUnit = 4503599627370496.0;  // 2^52: a listed weight as a whole number
@@ -212,9 +214,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   // of a search in the list, 8 bits a turn: weights in three parts whose sums over the list fit 32 bits each (one
   // add of 64 bits is a loop of compare-and-swap, and most listed keys share their upper digits)
   __shared__ uint32_t digits[4][3][256];
-  // a list of a token a thread: keys and weights
-  __shared__ __align__(16) uint32_t ranked[kThreads];
-  __shared__ __align__(16) unsigned long long ranked_w[kThreads];
+  // a short list: keys and weights
+  __shared__ __align__(16) uint32_t ranked[kRanked];
+  __shared__ __align__(16) unsigned long long ranked_w[kRanked];
   double* blk_mass = reinterpret_cast<double*>(smem);                       // [per_cta]
   uint32_t* blk_ties = reinterpret_cast<uint32_t*>(blk_mass + p.per_cta);   // [per_cta]
   float* blk_top = reinterpret_cast<float*>(blk_ties + p.per_cta);          // [per_cta] largest logit
@@ -597,8 +599,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       }
     }
     listed_n = n;
-    if (n <= kThreads) {
-      ranked[tid] = mine[0];
+    if (n <= kRanked) {
+      if (tid < kRanked) ranked[tid] = mine[0];
       __syncthreads();
     }
     return n;
@@ -609,8 +611,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   // weigh less than the goal.
   auto search = [&](const uint64_t (&w)[kList / kThreads], uint64_t extra, uint64_t goal, uint32_t& t, uint64_t& above,
                     uint64_t& equal) {
-    if (listed_n <= kThreads) {  // each thread looks at all of them for its own
-      ranked_w[tid] = w[0];
+    if (listed_n <= kRanked) {  // each thread looks at all of them for its own
+      if (tid < kRanked) ranked_w[tid] = w[0];
       if (tid == 0) sh.found = 0;
       __syncthreads();
       if (mine[0]) {
@@ -639,10 +641,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
     }
     const uint32_t differ = list_lo ^ list_hi;
     int bits = differ ? 32 - __clz(differ) : 1;  // the bits above are common to all
+    // 16-bit logits: the low bits follow from the upper ones (all 0, or all 1 below zero)
+    constexpr int kEnd = std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 13 : 16;
+    bits = max(bits, kEnd + 1);
     t = list_hi;
     above = equal = 0;
-    for (int turn = 0; bits > 0; ++turn) {
-      const int d = min(bits, 8), shift = bits - d;
+    for (int turn = 0; bits > kEnd; ++turn) {
+      const int d = min(bits - kEnd, 8), shift = bits - d;
       auto add = [&](uint32_t key, uint64_t e) {
         if (e && (bits == 32 || key >> bits == t >> bits)) {
           const uint32_t digit = key >> shift & 255u >> (8 - d), low = (uint32_t)e & 0x1fffff, mid = (uint32_t)(e >> 21) & 0x1fffff;
@@ -685,6 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       t = (bits == 32 ? 0u : t >> bits << bits) | digit << shift;
       bits = shift;
     }
+    if (kEnd && !(t & 0x80000000u)) t |= (1u << kEnd) - 1;
     return true;
   };
 
@@ -942,12 +948,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
         const double e = weight(v[i]);
         if (v[i] >= from) s2[i & 1] += e;
       }
+      s = s2[0] + s2[1];
       if (tau) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) n += v[i] == v_tau;
         n = __reduce_add_sync(0xffffffffu, n);
       }
-      s = warp_reduce(s2[0] + s2[1], Sum());
+      s = warp_reduce(s, Sum());
     }
     if (lane == 0) {
       blk_mass[blk] = s;
