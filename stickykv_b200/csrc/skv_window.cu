@@ -1,37 +1,18 @@
 // skv_window_attention: attention with a sliding window and first tokens that
-// stay visible (argument checks, dispatch and the portable kernel).
+// stay visible: argument checks and dispatch.
 //
 // Query at slot p of a row whose tokens sit in [start, end) sees key j when
 //   start <= j <= p < end and (j - start < sinks or p - j < window),
 // i.e. the runs [start, min(start + sinks, p + 1)) and
 // [max(start + sinks, p - window + 1, start), p].
-#include "skv_window_rows.cuh"
+#include "skv_window.cuh"
 
 namespace skv {
 int window_few(const WindowParams& p, int dtype, cudaStream_t stream);
+int window_f32(const WindowParams& p, cudaStream_t stream);
 bool window_many_supported(const WindowParams& p);
 int window_many(const WindowParams& p, int dtype, cudaStream_t stream);
 namespace {
-
-template <typename T, int D>
-__global__ void __launch_bounds__(128) window_rows_kernel(const __grid_constant__ WindowParams p) {
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
-  if (i >= p.T) return;
-  window_one_row<T, D>(p, window_row(p, b), b, h, i, threadIdx.x & 31, 0, D);
-}
-
-template <typename T>
-int launch_rows(const WindowParams& p, cudaStream_t stream) {
-  const dim3 grid(ceil_div(p.T, 4), p.Hq, p.B);
-  switch (p.D) {
-    case 16: window_rows_kernel<T, 16><<<grid, 128, 0, stream>>>(p); break;
-    case 32: window_rows_kernel<T, 32><<<grid, 128, 0, stream>>>(p); break;
-    case 64: window_rows_kernel<T, 64><<<grid, 128, 0, stream>>>(p); break;
-    default: window_rows_kernel<T, 128><<<grid, 128, 0, stream>>>(p); break;
-  }
-  SKV_CHECK_LAUNCH();
-  return SKV_OK;
-}
 
 int check_window(const skv_window_args* a) {
   if (!a) return SKV_ERR_INVALID_ARG;
@@ -80,7 +61,7 @@ extern "C" int skv_window_attention(const skv_window_args* a, void* stream) {
   p.sinks = a->sinks < a->k_slots ? a->sinks : a->k_slots;
   p.scaling = a->scaling;
   const cudaStream_t s = (cudaStream_t)stream;
-  if (a->dtype == SKV_F32) return launch_rows<float>(p, s);
+  if (a->dtype == SKV_F32) return window_f32(p, s);
   if ((int64_t)p.T * (p.Hq / p.Hkv) > 64 && window_many_supported(p)) return window_many(p, a->dtype, s);
   return window_few(p, a->dtype, s);
 }

@@ -21,7 +21,7 @@
 // Splits of one row group are the blocks of one cluster and join through
 // distributed shared memory: one launch, no workspace.
 #include "skv_mma.cuh"
-#include "skv_window_rows.cuh"
+#include "skv_window_join.cuh"
 
 namespace skv {
 namespace {
@@ -39,27 +39,15 @@ __device__ __forceinline__ void load_regs(uint32_t* dst, const void* src) {
   for (int i = 0; i < N; ++i) dst[i] = v.r[i];
 }
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-
 template <typename T, int D, int NT>
 struct FewCfg {
   static constexpr int kRows = 8 * NT;
   // head_dim 128 holds twice the registers: 12 warps an SM in three blocks (8 in two for 16 rows) instead of 16 in two
   static constexpr int kWarps = D == 128 ? 4 : 8;
   static constexpr int kBlocks = D == 128 && NT == 1 ? 3 : 2;
-  static constexpr int kPitch = D + 4;                       // floats a partial row (16-byte rows, banks apart)
-  static constexpr size_t kPart = (size_t)kWarps * kRows * kPitch * 4;
-  static constexpr size_t kStat = (size_t)(kWarps + 1) * kRows * 2 * 4;
-  static constexpr size_t kSmem = kPart + kStat;
+  static constexpr int kPitch = window_pitch(D);
+  static constexpr size_t kPart = window_part_bytes(D, kRows, kWarps);
+  static constexpr size_t kSmem = kPart + window_stat_bytes(kRows, kWarps);
 };
 
 template <typename T, int D, int NT>
@@ -278,113 +266,14 @@ __global__ void __launch_bounds__(FewCfg<T, D, NT>::kWarps * 32, FewCfg<T, D, NT
           *reinterpret_cast<float2*>(mine + r * C::kPitch + 8 * VC * c + VC * i8 + 2 * h) =
               make_float2(o[n][c * VR + h][e], o[n][c * VR + h][2 + e]);
     }
-  __syncthreads();
-  // the block's warps join into warp 0's place
-  const int n_out = rows * D;
-  for (int x = threadIdx.x; x < n_out; x += kWarps * 32) {
-    const int r = x / D, d = x % D;
-    float mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, stat[w * C::kRows + r]);
-    float sum = 0.f, val = 0.f;
-    if (mx != -INFINITY) {
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(stat[w * C::kRows + r] - mx);
-        sum += f * stat[(kWarps + 1 + w) * C::kRows + r];
-        val += f * part[(size_t)w * C::kRows * C::kPitch + r * C::kPitch + d];
-      }
-    }
-    part[r * C::kPitch + d] = val;
-    if (d == 0) {
-      stat[kWarps * C::kRows + r] = mx;
-      stat[(2 * kWarps + 1) * C::kRows + r] = sum;
-    }
-  }
-  if (splits > 1) cluster_sync();
-  else __syncthreads();
-  // and the cluster's blocks: each writes every splits-th row slice
-  bool repair = false;
-  const int per = ceil_div(n_out, splits);
-  const uint32_t s_part = smem_u32(part), s_stat = smem_u32(stat);
-  for (int y = threadIdx.x; y < per; y += kWarps * 32) {
-    const int x = split * per + y;
-    if (x >= n_out) break;
-    const int r = x / D, d = x % D;
-    float mx = -INFINITY, sum = 0.f, val = 0.f;
-    if (splits == 1) {
-      sum = stat[(2 * kWarps + 1) * C::kRows + r];
-      val = part[r * C::kPitch + d];
-    } else {
-      for (int z = 0; z < splits; ++z) {
-        const float mz = ld_cluster(s_stat + (kWarps * C::kRows + r) * 4, z);
-        const float lz = ld_cluster(s_stat + ((2 * kWarps + 1) * C::kRows + r) * 4, z);
-        const float vz = ld_cluster(s_part + (r * C::kPitch + d) * 4, z);
-        if (mz == -INFINITY) continue;
-        const float mn = fmaxf(mx, mz), f0 = ex2(mx - mn), f1 = ex2(mz - mn);
-        sum = sum * f0 + lz * f1;
-        val = val * f0 + vz * f1;
-        mx = mn;
-      }
-    }
-    const float res = sum == 0.f ? 0.f : val / sum;
-    repair |= !(fabsf(res) < INFINITY);
-    const int rr = r0 + r;
-    st_f32((T*)p.out + (((int64_t)b * p.T + rr / G) * p.Hq + kh * G + rr % G) * D + d, res);
-  }
-  // a key that is not finite reaches the rows that do not see it as 0 * inf:
-  // rows that come out not finite are done again key by key
-  const int again = __syncthreads_or(repair);
-  if (again) {
-    for (int r = warp; r < rows; r += kWarps) {
-      const int rr = r0 + r;
-      if (r * D / per <= split && (r * D + D - 1) / per >= split)
-        window_one_row<T, D>(p, row, b, kh * G + rr % G, rr / G, lane, split * per - r * D, (split + 1) * per - r * D);
-    }
-  }
-  if (splits > 1) cluster_sync();  // no block leaves while others read its share
+  window_join<T, D, C::kRows, kWarps>(p, row, b, kh, r0, rows, split, splits, part, stat);
 }
 
 template <typename T, int D, int NT>
 int launch_few(const WindowParams& p, cudaStream_t stream) {
   using C = FewCfg<T, D, NT>;
-  static std::atomic<uint32_t> done{0}, wide{0};
-  const auto kernel = window_few_kernel<T, D, NT>;
-  max_smem_once(done, kernel, (int)C::kSmem);
-  const int G = p.Hq / p.Hkv;
-  const int64_t groups = ceil_div64((int64_t)p.T * G, C::kRows);
-  const int64_t blocks = groups * p.Hkv * p.B;
-  const int64_t tiles = ceil_div64(std::min<int64_t>(p.S, (int64_t)p.sinks + p.window + ceil_div(C::kRows, G)), 16);
-  // splits: as long as all blocks are resident at once and every warp has a tile
-  int splits = 1;
-  while (splits < 16 && blocks * splits * 2 <= C::kBlocks * 148 && (int64_t)splits * 2 * C::kWarps <= tiles) splits *= 2;
-  if (groups * splits > 0x7fffffff) return SKV_ERR_UNSUPPORTED;
-  if (splits > 8) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const uint32_t bit = dev < 32 ? 1u << dev : 0u;
-    if (!bit || !(wide.load(std::memory_order_relaxed) & bit)) {
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      wide.fetch_or(bit, std::memory_order_relaxed);
-    }
-  }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(groups * splits), p.Hkv, p.B);
-  cfg.blockDim = dim3(C::kWarps * 32);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = splits;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, splits);
-  if (e != cudaSuccess) {
-    set_cuda_error(e);
-    return SKV_ERR_CUDA;
-  }
-  return SKV_OK;
+  static WindowFewState state;
+  return launch_window_few(p, window_few_kernel<T, D, NT>, state, C::kRows, C::kWarps, C::kBlocks, C::kSmem, stream);
 }
 
 template <typename T>

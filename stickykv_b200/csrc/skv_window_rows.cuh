@@ -1,6 +1,6 @@
-// One row of window attention by one warp, key by key: the portable kernel's
-// body, and what the tensor-core kernels fall back to for rows that come out
-// not finite (so that keys a row does not see never reach it).
+// One row of window attention by one warp, key by key: what the tensor-core
+// kernels fall back to for rows that come out not finite (so that keys a row
+// does not see never reach it).
 #pragma once
 
 #include "skv_window.cuh"

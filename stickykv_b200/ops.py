@@ -18,10 +18,39 @@ import torch
 from torch import Tensor
 
 from ._lib import RotaryArgs, SampleArgs, WindowArgs, check, lib
-from .cache import _DT, _on, _stream
+from .cache import _DT, _cur_dev, _on, _raw_stream, _stream
 
 _I3 = C.c_int64 * 3
 _I2 = C.c_int64 * 2
+
+# Arguments of calls that passed every check and needed no copy of an input, by
+# what was checked: shapes, strides, types and settings, never an address or a
+# tensor.  A decode step makes the same few calls again and again; from here
+# each costs about half its Python time (a copy of the struct with this call's
+# pointers filled in).
+_PLANS: Dict[tuple, C.Structure] = {}
+
+
+def _keep(key: tuple, args: C.Structure) -> None:
+    if len(_PLANS) >= 1024:
+        _PLANS.clear()
+    _PLANS[key] = type(args).from_buffer_copy(args)
+
+
+def _meta(t: Optional[Tensor]) -> Optional[tuple]:
+    return None if t is None else (t.dtype, t.shape, t.stride())
+
+
+def _ready(index: int, *tensors: Optional[Tensor]) -> bool:
+    """All on GPU ``index``, which is the current one, and none asks for
+    gradients: nothing is left to check but the plan's key."""
+    if index < 0 or _cur_dev is None or _raw_stream is None or _cur_dev() != index:
+        return False
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and (t.get_device() != index or (grad and t.requires_grad)):
+            return False
+    return True
 
 
 def _same_device(what: str, device: torch.device, **tensors: Optional[Tensor]) -> None:
@@ -142,6 +171,23 @@ def apply_rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, inv_fr
     rotated channels; ``inverse`` turns back (and still multiplies by
     ``scale``).  ``out`` gives the outputs' tensors; each may be its own input
     (in place) and must otherwise not overlap any input."""
+    plan_key = None
+    if out is None:
+        index = query.get_device()
+        if _ready(index, query, key, positions, inv_freq):
+            plan_key = ("rotary", query.dtype, query.shape, query.stride(), _meta(key), _meta(positions), _meta(inv_freq),
+                        interleaved, scale, inverse)
+            plan = _PLANS.get(plan_key)
+            if plan is not None:
+                a = RotaryArgs.from_buffer_copy(plan)
+                q_out, k_out = torch.empty_like(query), None
+                a.q, a.q_out = query.data_ptr(), q_out.data_ptr()
+                if key is not None:
+                    k_out = torch.empty_like(key)
+                    a.k, a.k_out = key.data_ptr(), k_out.data_ptr()
+                a.positions, a.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
+                check(lib().skv_rotary(C.byref(a), _raw_stream(index)), "skv_rotary")
+                return q_out, k_out
     _same_device("apply_rotary", query.device, key=key, positions=positions, inv_freq=inv_freq)
     _no_grad("apply_rotary", query, key, positions, inv_freq)
     if query.dim() != 4 or (key is not None and key.dim() != 4):
@@ -156,6 +202,7 @@ def apply_rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, inv_fr
     r = 2 * inv_freq.shape[0]
     if not 0 < r <= D:
         raise ValueError(f"apply_rotary: inv_freq has {r // 2} pairs, a head {D} channels")
+    given = positions
     if positions.dtype != torch.int64:
         if positions.dtype != torch.int32:
             raise ValueError(f"apply_rotary: positions must be int64 or int32, got {positions.dtype}")
@@ -197,6 +244,9 @@ def apply_rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, inv_fr
     Hkv = 0 if k is None else k.shape[1]
     if Hkv == 0:
         k = None
+    if plan_key is not None and not (q is query and (key is None or k is key) and qo is q_out and ko is k_out
+                                     and positions is given and inv_freq.is_contiguous()):
+        plan_key = None
     inv_freq = inv_freq.contiguous()
     qs, qos = q.stride(), qo.stride()
     ks, kos = (k.stride(), ko.stride()) if k is not None else ((0,) * 4, (0,) * 4)
@@ -206,6 +256,8 @@ def apply_rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, inv_fr
                    _I2(ps_b, positions.stride(-1)), inv_freq.data_ptr())
     with _on(q.device):
         check(lib().skv_rotary(C.byref(a), _stream(q.device)), "skv_rotary")
+    if plan_key is not None:
+        _keep(plan_key, a)
     if qo is not q_out:
         q_out.copy_(qo)
     if ko is not k_out:
@@ -252,6 +304,28 @@ def sink_window_attention(query: Tensor, key: Tensor, value: Tensor, *, window: 
     ``ends`` and zero ``query_slots``, a decode step over a preallocated cache
     ``ends``.  A query that sees no key (padding) gets zeros; what a query does
     not see never reaches its output, whatever it holds."""
+    plan_key = None
+    if out is None:
+        index = query.get_device()
+        if _ready(index, query, key, value, starts, ends, query_slots):
+            qp, kp, vp = query.data_ptr(), key.data_ptr(), value.data_ptr()
+            if not (qp | kp | vp) & 15:
+                plan_key = ("window", query.dtype, query.shape, query.stride(), _meta(key), _meta(value), _meta(starts),
+                            _meta(ends), _meta(query_slots), window, sinks, scaling)
+                plan = _PLANS.get(plan_key)
+                if plan is not None:
+                    a = WindowArgs.from_buffer_copy(plan)
+                    out = torch.empty((a.batch, a.q_tokens, a.num_q_heads, a.head_dim), dtype=query.dtype,
+                                      device=query.device)
+                    a.q, a.k, a.v, a.out = qp, kp, vp, out.data_ptr()
+                    if starts is not None:
+                        a.starts = starts.data_ptr()
+                    if ends is not None:
+                        a.ends = ends.data_ptr()
+                    if query_slots is not None:
+                        a.query_slots = query_slots.data_ptr()
+                    check(lib().skv_window_attention(C.byref(a), _raw_stream(index)), "skv_window_attention")
+                    return out
     _same_device("sink_window_attention", query.device, key=key, value=value, starts=starts, ends=ends,
                  query_slots=query_slots, out=out)
     _no_grad("sink_window_attention", query, key, value, out)
@@ -297,6 +371,8 @@ def sink_window_attention(query: Tensor, key: Tensor, value: Tensor, *, window: 
                    None if query_slots is None else query_slots.data_ptr())
     with _on(q.device):
         check(lib().skv_window_attention(C.byref(a), _stream(q.device)), "skv_window_attention")
+    if plan_key is not None and q is query and k is key and v is value:
+        _keep(plan_key, a)
     return out
 
 
@@ -322,6 +398,24 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
     or below 0 or NaN is greedy, a top_k at or below 0, a top_p from 1 on and
     a min_p at or below 0 cut nothing, a top_p at or below 0 keeps one token.
     The largest token is always kept.  V is at most 4,194,304."""
+    plan_key = None
+    if out is None:
+        index = logits.get_device()
+        tensors = [None if s.__class__ in (int, float) else s if torch.is_tensor(s) else None
+                   for s in (temperature, top_k, top_p, min_p)]
+        if _ready(index, logits, uniform, *tensors):
+            plan_key = ("sample", logits.dtype, logits.shape, logits.stride(), _meta(uniform)) + tuple(
+                s if t is None else _meta(t) for s, t in zip((temperature, top_k, top_p, min_p), tensors))
+            plan = _PLANS.get(plan_key)
+            if plan is not None:
+                a = SampleArgs.from_buffer_copy(plan)
+                out = torch.empty((a.batch,), dtype=torch.int64, device=logits.device)
+                a.logits, a.uniform, a.tokens = logits.data_ptr(), uniform.data_ptr(), out.data_ptr()
+                for name, t in zip(("temperatures", "top_ks", "top_ps", "min_ps"), tensors):
+                    if t is not None:
+                        setattr(a, name, t.data_ptr())
+                check(lib().skv_sample(C.byref(a), _raw_stream(index)), "skv_sample")
+                return out
     _same_device("sample_tokens", logits.device, uniform=uniform, out=out)
     _no_grad("sample_tokens", logits, uniform)
     if logits.dim() != 2 or logits.shape[1] == 0:
@@ -364,4 +458,6 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
                    uniform.data_ptr(), arrays[0], arrays[1], arrays[2], arrays[3], out.data_ptr())
     with _on(x.device):
         check(lib().skv_sample(C.byref(a), _stream(x.device)), "skv_sample")
+    if plan_key is not None and x is logits:
+        _keep(plan_key, a)
     return out
