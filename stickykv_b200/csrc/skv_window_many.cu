@@ -7,8 +7,8 @@
 // first tokens (rounded up to 8) and the window, which one sequence of 128-key
 // tiles covers: a few first tokens share a tile with the window's beginning.
 //
-//   warp 9         TMA: Q once, then K and V tiles through a ring
-//   warp 8         one thread issues the MMAs:  S_t = Q_t K^T,  O_t += P_t V
+//   warp 9         TMA (10 and 11 complete the warpgroup): Q once, then K and V tiles through a ring
+//   warp 8         issues the MMAs:  S_t = Q_t K^T,  O_t += P_t V
 //   warps 0-3/4-7  softmax of tile 0/1, a thread a row: S from tensor memory,
 //                  P = exp2(S - m) back into S's columns as the second MMA's A
 //                  operand; the running maximum m moves only when it is passed
@@ -31,14 +31,18 @@ using mma::Op;
 using mma::smem_u32;
 
 constexpr int kRows = 128;
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
+constexpr int kPoly = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D> struct ManyCfg {
   static constexpr int kTile = kRows * D * 2;
   static constexpr int kHalf = kRows * 128;                  // 64 channels of a tile
   static constexpr int kStages = D == 128 ? 4 : 8;           // K and V tiles in turn
-  static constexpr int kBars = 1 + 2 * kStages + 6;
+  static constexpr int kBars = 1 + 2 * kStages + 10;
+  // head_dim 64 leaves room for P beside S, so that the next S need not wait for this P's product
+  static constexpr bool kApart = D == 64;
+  static constexpr int kO = 2 * kRows, kP = kApart ? 2 * kRows + 2 * D : 0, kPStep = kApart ? 64 : kRows;  // columns
   static constexpr size_t kSmem = (size_t)(2 + kStages) * kTile + kBars * 8 + 16 + 1024;  // + alignment
 };
 
@@ -56,8 +60,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t sQ = base, sR = base + 2 * C::kTile, bars = sR + C::kStages * C::kTile;
   const uint32_t bQ = bars, bFull = bars + 8, bFree = bFull + 8 * C::kStages, bS = bFree + 8 * C::kStages,
-                 bP = bS + 16, bO = bP + 16, sAddr = bO + 16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+                 bL = bS + 16, bP = bL + 16, bP2 = bP + 16, bO = bP2 + 16, sAddr = bO + 16;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kh = blockIdx.y, b = blockIdx.z;
   const int G = p.Hq / p.Hkv, TQ = kRows / G;                // tokens of a tile
   const int i0 = (gridDim.x - 1 - blockIdx.x) * 2 * TQ;      // first token; the last tokens first
@@ -100,7 +104,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < 2 * C::kStages; ++s) bar_init(bFull + 8 * s, 1);
     for (int t = 0; t < 2; ++t) {
       bar_init(bS + 8 * t, 1);
+      bar_init(bL + 8 * t, kRows);
       bar_init(bP + 8 * t, kRows);
+      bar_init(bP2 + 8 * t, kRows);
       bar_init(bO + 8 * t, 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -112,7 +118,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(tmem) : "r"(sAddr));
   bool lost = false;  // a wait ran out: the rest is not waited for, and the rows are done again key by key
 
-  if (warp == 9) {
+  // 168 registers a thread at launch, three warpgroups: 2 x 208 + 80 of the 504 they share
+  if (warp >= 8) {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n" ::);
+   if (warp == 9) {
     if (lane == 0 && n > 0) {
       const int nq = i0 + TQ < p.T ? 2 : 1;
       bar_expect(bQ, nq * G * TQ * D * 2);
@@ -141,54 +150,75 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-  } else if (warp == 8) {
-    if (lane == 0 && n > 0) {
+   } else if (warp == 8) {
+    if (n > 0) {
       auto wait = [&](uint32_t bar, uint32_t parity) {
         if (!lost && !bar_wait(bar, parity)) lost = true;
+        lost = __any_sync(0xffffffffu, lost);
         fence_after();
       };
       auto full = [&](int x) { wait(bFull + 8 * (x % C::kStages), (x / C::kStages) & 1); };
       auto issue_s = [&](int t, int j) {
-        const uint32_t q = sQ + t * C::kTile, k = sR + (2 * j % C::kStages) * C::kTile;
+        const uint64_t q = desc_k(sQ + t * C::kTile), k = desc_k(sR + (2 * j % C::kStages) * C::kTile);
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) {
-          const uint32_t off = (e >> 2) * C::kHalf + (e & 3) * 32;
-          mma_ss(tmem + t * kRows, desc_k(q + off), desc_k(k + off), kIdS, e > 0);
+          const uint32_t off = ((e >> 2) * C::kHalf + (e & 3) * 32) >> 4;
+          mma_ss(tmem + t * kRows, q + off, k + off, kIdS, e > 0);
         }
         commit(bS + 8 * t);
       };
+      // P's first three quarters are there before the last: the product begins with them
       auto issue_o = [&](int t, int j) {
-        const uint32_t v = sR + ((2 * j + 1) % C::kStages) * C::kTile;
+        const uint64_t v = desc_mn(sR + ((2 * j + 1) % C::kStages) * C::kTile, C::kHalf);
+        const uint32_t first = j > lo[t], par = (j - lo[t]) & 1;
+        wait(bP + 8 * t, par);
+        full(2 * j + 1);
 #pragma unroll
-        for (int e = 0; e < kRows / 16; ++e)
-          mma_ts(tmem + 2 * kRows + t * D, tmem + t * kRows + 8 * e, desc_mn(v + e * 16 * 128, C::kHalf), kIdO,
-                 j > lo[t] || e > 0);
+        for (int e = 0; e < kRows / 16; ++e) {
+          if (e == 6) wait(bP2 + 8 * t, par);
+          mma_ts(tmem + C::kO + t * D, tmem + C::kP + t * C::kPStep + 8 * e, v + (e * 16 * 128 >> 4), kIdO, e > 0 ? 1u : first);
+        }
         commit(bO + 8 * t);
+      };
+      auto next_s = [&](int t, int j) {
+        if (j + 1 >= lo[t] && j + 1 < hi[t]) {
+          if (C::kApart && j >= lo[t]) wait(bL + 8 * t, (j - lo[t]) & 1);  // this S has been read
+          full(2 * j + 2);
+          issue_s(t, j + 1);
+        }
       };
       wait(bQ, 0);
       full(0);
+#pragma unroll
       for (int t = 0; t < 2; ++t)
         if (lo[t] == 0 && hi[t] > 0) issue_s(t, 0);
       commit(bFree);
       for (int j = 0; j < n; ++j) {
-        for (int t = 0; t < 2; ++t) {
-          if (j >= lo[t] && j < hi[t]) {
-            wait(bP + 8 * t, (j - lo[t]) & 1);
-            full(2 * j + 1);
-            issue_o(t, j);
-          }
-          if (j + 1 >= lo[t] && j + 1 < hi[t]) {
+        if (C::kApart) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) next_s(t, j);
+          if (j + 1 < n) {
             full(2 * j + 2);
-            issue_s(t, j + 1);
+            commit(bFree + 8 * ((2 * j + 2) % C::kStages));
           }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (j >= lo[t] && j < hi[t]) issue_o(t, j);
+          if (!C::kApart) next_s(t, j);
         }
         full(2 * j + 1);
         commit(bFree + 8 * ((2 * j + 1) % C::kStages));
-        if (j + 1 < n) commit(bFree + 8 * ((2 * j + 2) % C::kStages));
+        if (!C::kApart && j + 1 < n) {
+          full(2 * j + 2);
+          commit(bFree + 8 * ((2 * j + 2) % C::kStages));
+        }
       }
     }
     __syncwarp();
+   }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n" ::);
     const int t = warp >> 2, rl = threadIdx.x & 127;
     const int token = i0 + t * TQ + rl / G, h = kh * G + rl % G;
     const bool real = rl < TQ * G && token < p.T;            // a row of the output
@@ -205,7 +235,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const float sl2 = p.scaling * kLog2e;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t tS = tmem + lanes + t * kRows, tO = tmem + lanes + 2 * kRows + t * D;
+    const uint32_t tS = tmem + lanes + t * kRows, tO = tmem + lanes + C::kO + t * D;
+    const uint32_t tP = tmem + lanes + C::kP + t * C::kPStep;
     float m = -INFINITY, l = 0.f;
     for (int j = lo[t]; j < hi[t]; ++j) {
       const int it = j - lo[t], v0 = j * kRows;
@@ -216,11 +247,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < 4; ++c) ld32(r + 32 * c, tS + 32 * c);
       ld_wait();
       const bool whole = (rb0 <= v0 && v0 + kRows <= rb1) || v0 + kRows <= ra;
+      if (C::kApart) {
+        fence_before();
+        bar_arrive(bL + 8 * t);
+      }
       float mx = -INFINITY;
-      if (__all_sync(0xffffffffu, whole)) {
+      const bool all_whole = __all_sync(0xffffffffu, whole);
+      if (all_whole) {
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(r[i]));
+        for (int i = 0; i < kRows; i += 2)
+          m4[(i >> 1) & 3] = fmaxf(m4[(i >> 1) & 3], fmaxf(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       } else {
         const int ea = ra - v0, e0 = rb0 - v0, e1 = rb1 - v0;
@@ -264,19 +301,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const float mm = m == -INFINITY ? 0.f : m;
-      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+      // P = exp2(S - m), a pair at a time; where nothing is masked, one pair of kPoly by arithmetic beside the
+      // exponential unit, the tighter bound
+      const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(-mm, -mm);
+      float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      auto weigh = [&](auto poly, int i) {
+        float2 x = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), scale2, shift2);
+        if (poly.value && (i >> 1) % kPoly == kPoly - 1) x = exp2_poly2(x);
+        else x = make_float2(ex2(x.x), ex2(x.y));
+        sum2[(i >> 1) & 1] = add2(sum2[(i >> 1) & 1], x);
+        r[i >> 1] = Op<T>::pack(x.x, x.y);
+      };
+      auto weigh_all = [&](auto poly) {
 #pragma unroll
-      for (int i = 0; i < kRows; i += 2) {
-        const float x = ex2(fmaf(__uint_as_float(r[i]), sl2, -mm)), y = ex2(fmaf(__uint_as_float(r[i + 1]), sl2, -mm));
-        s4[(i >> 1) & 3] += x + y;
-        r[i >> 1] = Op<T>::pack(x, y);
-      }
-      l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-      st32(tS, r);
-      st32(tS + 32, r + 32);
+        for (int i = 0; i < 96; i += 2) weigh(poly, i);
+        // the product of the tile before has read its P
+        if (C::kApart && it > 0 && !lost && !bar_wait(bO + 8 * t, (it - 1) & 1)) lost = true;
+        st32(tP, r);
+        st16(tP + 32, r + 32);
+        st_wait();
+        fence_before();
+        bar_arrive(bP + 8 * t);
+#pragma unroll
+        for (int i = 96; i < kRows; i += 2) weigh(poly, i);
+      };
+      if (all_whole) weigh_all(std::true_type());
+      else weigh_all(std::false_type());
+      l += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
+      st16(tP + 48, r + 48);
       st_wait();
       fence_before();
-      bar_arrive(bP + 8 * t);
+      bar_arrive(bP2 + 8 * t);
     }
     // O / l
     const int last = hi[t] - lo[t] - 1;

@@ -9,7 +9,7 @@ namespace skv {
 
 // Lanes over the channels, online softmax in fp32.  Writes channels [d0, d1).
 template <typename T, int D>
-__device__ __noinline__ void window_one_row(const WindowParams& p, const WindowRow& row, int b, int h, int i,
+__device__ __forceinline__ void window_one_row(const WindowParams& p, const WindowRow& row, int b, int h, int i,
                                             int lane, int d0, int d1) {
   constexpr int E = D < 32 ? 1 : D / 32;
   const int pos = row.first + i, kh = h / (p.Hq / p.Hkv);
