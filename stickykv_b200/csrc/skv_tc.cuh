@@ -132,25 +132,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-// 2^x by arithmetic, for x up to 30 or so (below -126: 2^-126 or so): 2^n from
-// the rounding to whole numbers, 2^f, |f| <= 1/2, by the polynomial that
-// interpolates it at the 5 Chebyshev nodes (off by 3e-6 at most)
-__device__ __forceinline__ float2 exp2_poly2(float2 x) {
-  const float kMagic = 12582912.f;  // 1.5 * 2^23
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 t = add2(x, make_float2(kMagic, kMagic));
-  const float2 n = add2(t, make_float2(-kMagic, -kMagic));
-  const float2 f = add2(x, make_float2(-n.x, -n.y));
-  auto both = [](float c) { return make_float2(c, c); };
-  float2 e = fma2(both(0.00966636852f), f, both(0.0559219758f));
-  e = fma2(e, f, both(0.24022349f));
-  e = fma2(e, f, both(0.693121045f));
-  e = fma2(e, f, both(1.f));
-  return make_float2(__uint_as_float(__float_as_uint(e.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(e.y) + (__float_as_uint(t.y) << 23)));
-}
-
 // Host: a tiled map of 16-bit elements with 64-element (128-byte) swizzled
 // rows.  dims/strides (bytes, of dims 1..) innermost first.
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

@@ -32,7 +32,6 @@ using mma::smem_u32;
 
 constexpr int kRows = 128;
 constexpr int kThreads = 384;
-constexpr int kPoly = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D> struct ManyCfg {
@@ -99,7 +98,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(sAddr));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
   }
-  if (threadIdx.x == 0) {
+  auto load_kv = [&](int x) {  // K_0 V_0 K_1 V_1 .. of the ring
+    const int s = x % C::kStages, j = x >> 1, v0 = j * kRows;
+    const bool val = x & 1;
+    const uint32_t dst = sR + s * C::kTile, bar = bFull + 8 * s;
+    const CUtensorMap *map = val ? &maps.v : &maps.k, *map8 = val ? &maps.v8 : &maps.k8;
+    const int64_t* st = val ? p.vs : p.ks;
+    const int ch = st[1] ? kh : 0, cb = st[0] ? b : 0;  // shared by all heads or rows: one entry in the map
+    bar_expect(bar, C::kTile);
+    if (v0 + kRows <= A8 || v0 >= A8) {
+      const int slot = v0 >= A8 ? w0 + v0 - A8 : a0 + v0;
+      for (int h = 0; h < D / 64; ++h) tma4(dst + h * C::kHalf, map, bar, 64 * h, slot, ch, cb);
+    } else {  // both runs in one tile: 8 rows at a time
+      for (int r = 0; r < kRows; r += 8) {
+        const int slot = v0 + r >= A8 ? w0 + v0 + r - A8 : a0 + v0 + r;
+        for (int h = 0; h < D / 64; ++h) tma4(dst + h * C::kHalf + r * 128, map8, bar, 64 * h, slot, ch, cb);
+      }
+    }
+  };
+  if (warp == 9 && lane == 0) {
     bar_init(bQ, 1);
     for (int s = 0; s < 2 * C::kStages; ++s) bar_init(bFull + 8 * s, 1);
     for (int t = 0; t < 2; ++t) {
@@ -110,6 +127,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       bar_init(bO + 8 * t, 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    fence_proxy();
+    if (n > 0) {  // the queries and the first tile are on their way before the block has met
+      const int nq = i0 + TQ < p.T ? 2 : 1;
+      bar_expect(bQ, nq * G * TQ * D * 2);
+      for (int t = 0; t < nq; ++t)
+        for (int h = 0; h < D / 64; ++h)
+          tma5(sQ + t * C::kTile + h * C::kHalf, &maps.q, bQ, 64 * h, 0, i0 + t * TQ, kh, p.qs[0] ? b : 0);
+      load_kv(0);
+      load_kv(1);
+    }
   }
   fence_before();
   __syncthreads();
@@ -122,32 +149,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= 8) {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n" ::);
    if (warp == 9) {
-    if (lane == 0 && n > 0) {
-      const int nq = i0 + TQ < p.T ? 2 : 1;
-      bar_expect(bQ, nq * G * TQ * D * 2);
-      for (int t = 0; t < nq; ++t)
-        for (int h = 0; h < D / 64; ++h)
-          tma5(sQ + t * C::kTile + h * C::kHalf, &maps.q, bQ, 64 * h, 0, i0 + t * TQ, kh, p.qs[0] ? b : 0);
-      for (int x = 0; x < 2 * n; ++x) {  // K_0 V_0 K_1 V_1 ..
-        const int s = x % C::kStages, use = x / C::kStages, j = x >> 1, v0 = j * kRows;
-        if (use > 0 && !lost && !bar_wait(bFree + 8 * s, (use - 1) & 1)) lost = true;
-        if (lost) break;
-        const bool val = x & 1;
-        const uint32_t dst = sR + s * C::kTile, bar = bFull + 8 * s;
-        const CUtensorMap *map = val ? &maps.v : &maps.k, *map8 = val ? &maps.v8 : &maps.k8;
-        const int64_t* st = val ? p.vs : p.ks;
-        const int ch = st[1] ? kh : 0, cb = st[0] ? b : 0;  // shared by all heads or rows: one entry in the map
-        bar_expect(bar, C::kTile);
-        if (v0 + kRows <= A8 || v0 >= A8) {
-          const int slot = v0 >= A8 ? w0 + v0 - A8 : a0 + v0;
-          for (int h = 0; h < D / 64; ++h) tma4(dst + h * C::kHalf, map, bar, 64 * h, slot, ch, cb);
-        } else {  // both runs in one tile: 8 rows at a time
-          for (int r = 0; r < kRows; r += 8) {
-            const int slot = v0 + r >= A8 ? w0 + v0 + r - A8 : a0 + v0 + r;
-            for (int h = 0; h < D / 64; ++h)
-              tma4(dst + h * C::kHalf + r * 128, map8, bar, 64 * h, slot, ch, cb);
-          }
-        }
+    if (lane == 0) {
+      for (int x = 2; x < 2 * n; ++x) {
+        const int s = x % C::kStages, use = x / C::kStages;
+        if (use > 0 && !bar_wait(bFree + 8 * s, (use - 1) & 1)) break;
+        load_kv(x);
       }
     }
    } else if (warp == 8) {
@@ -251,22 +257,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_before();
         bar_arrive(bL + 8 * t);
       }
-      float mx = -INFINITY;
-      const bool all_whole = __all_sync(0xffffffffu, whole);
-      if (all_whole) {
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < kRows; i += 2)
-          m4[(i >> 1) & 3] = fmaxf(m4[(i >> 1) & 3], fmaxf(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
-        mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-      } else {
+      if (!__all_sync(0xffffffffu, whole)) {  // a bit for every column that the row sees
         const int ea = ra - v0, e0 = rb0 - v0, e1 = rb1 - v0;
+        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          if (!(i < ea || (i >= e0 && i < e1))) r[i] = __float_as_uint(-INFINITY);
-          mx = fmaxf(mx, __uint_as_float(r[i]));
+        for (int c = 0; c < kRows; c += 32) {
+          const uint32_t seen = below(ea - c) | (below(e1 - c) & ~below(e0 - c));
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(seen >> i & 1)) r[c + i] = __float_as_uint(-INFINITY);
         }
       }
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < kRows; i += 2)
+        m4[(i >> 1) & 3] = fmaxf(m4[(i >> 1) & 3], fmaxf(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
+      float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       // values of slots that no row sees may be anything: they become zeros
       if ((v0 < A8 && v0 + kRows > nA) || v0 + kRows > total) {
         const int x = 2 * j + 1, v = v0 + rl;
@@ -301,32 +307,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const float mm = m == -INFINITY ? 0.f : m;
-      // P = exp2(S - m), a pair at a time; where nothing is masked, one pair of kPoly by arithmetic beside the
-      // exponential unit, the tighter bound
+      // P = exp2(S - m), two of the multiply-adds an instruction (scalar ones: 7 % slower)
       const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(-mm, -mm);
       float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      auto weigh = [&](auto poly, int i) {
+      auto weigh = [&](int i) {
         float2 x = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), scale2, shift2);
-        if (poly.value && (i >> 1) % kPoly == kPoly - 1) x = exp2_poly2(x);
-        else x = make_float2(ex2(x.x), ex2(x.y));
+        x = make_float2(ex2(x.x), ex2(x.y));
         sum2[(i >> 1) & 1] = add2(sum2[(i >> 1) & 1], x);
         r[i >> 1] = Op<T>::pack(x.x, x.y);
       };
-      auto weigh_all = [&](auto poly) {
 #pragma unroll
-        for (int i = 0; i < 96; i += 2) weigh(poly, i);
-        // the product of the tile before has read its P
-        if (C::kApart && it > 0 && !lost && !bar_wait(bO + 8 * t, (it - 1) & 1)) lost = true;
-        st32(tP, r);
-        st16(tP + 32, r + 32);
-        st_wait();
-        fence_before();
-        bar_arrive(bP + 8 * t);
+      for (int i = 0; i < 96; i += 2) weigh(i);
+      // the product of the tile before has read its P
+      if (C::kApart && it > 0 && !lost && !bar_wait(bO + 8 * t, (it - 1) & 1)) lost = true;
+      st32(tP, r);
+      st16(tP + 32, r + 32);
+      st_wait();
+      fence_before();
+      bar_arrive(bP + 8 * t);
 #pragma unroll
-        for (int i = 96; i < kRows; i += 2) weigh(poly, i);
-      };
-      if (all_whole) weigh_all(std::true_type());
-      else weigh_all(std::false_type());
+      for (int i = 96; i < kRows; i += 2) weigh(i);
       l += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
       st16(tP + 48, r + 48);
       st_wait();
