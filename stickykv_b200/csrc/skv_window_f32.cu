@@ -5,14 +5,17 @@
 //   S (16 rows x 8 keys) = Q K^T,  O (16 rows x D) += P V
 // on mma.sync m16n8k8 with tf32 operands.  A float32 number is the sum of two
 // tf32 ones to 2^-22 of itself, so each product is three: high x high, high x
-// low, low x high; sums are 32-bit.  The orders of the contracted channels and
+// low, low x high.  The matrix unit cuts off what it adds up, always towards
+// zero, so a sum stays in it for a few products only (8 keys of O; of S the two
+// halves and the small cross terms apart) and goes on in rounded 32-bit
+// additions: all in it, 16000 keys came out 2e-6 off.  The orders of the contracted channels and
 // keys and of the output channels are free and chosen so that every lane loads
 // 4 neighbouring channels at once, and P's accumulator layout is the second
 // product's operand layout: no shared memory in the loop, no exchange.
 //
-// Bound: decode HBM (and the three-fold MMAs, level with it at 16 rows); prompts
-// the MMAs.  CUDA cores would take 4 D flops a pair at 75 TFLOP/s, this takes
-// 12 D at the tf32 rate of mma.sync, four times that.
+// Bound: the three-fold MMAs and the splitting of K and V beside them (decode of
+// 18 rows, 8 kv heads, 1305 keys, head_dim 128: 58 us, 3.3 TB/s of the cache's
+// bytes; a prompt of 8 x 1500 tokens, 64 heads of 128: 9.1 ms).
 #include "skv_window_join.cuh"
 
 namespace skv {
@@ -24,9 +27,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 4, kRows = 16;
 
 template <int D> struct F32Cfg {
-  static constexpr int kBlocks = D == 128 ? 2 : 4;  // of 4 warps an SM: 232 and 128 registers
+  static constexpr int kBlocks = D == 128 ? 2 : 4;  // of 4 warps an SM: 255 and 128 registers
   static constexpr size_t kPart = window_part_bytes(D, kRows, kWarps);
-  static constexpr size_t kSmem = kPart + window_stat_bytes(kRows, kWarps);
+  static constexpr size_t kStat = window_stat_bytes(kRows, kWarps);
+  static constexpr int kSteps = D / 8;              // of the first product
+  static constexpr size_t kSmem = kPart + kStat + (size_t)kSteps * 2 * 32 * 16;  // and the queries' operands
 };
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -35,8 +40,13 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t high(float x) { return __float_as_uint(x) & 0xffffe000u; }
-__device__ __forceinline__ uint32_t low(float x) { return __float_as_uint(x - __uint_as_float(high(x))); }
+// the two terms of a number, each to the nearest
+__device__ __forceinline__ uint32_t high(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t low(float x) { return high(x - __uint_as_float(high(x))); }
 
 template <int D>
 __global__ void __launch_bounds__(kWarps * 32, F32Cfg<D>::kBlocks)
@@ -74,21 +84,28 @@ __global__ void __launch_bounds__(kWarps * 32, F32Cfg<D>::kBlocks)
   const int parts = splits * kWarps, me = split * kWarps + warp;
   const int tile0 = (int)((int64_t)tiles * me / parts), tile1 = (int)((int64_t)tiles * (me + 1) / parts);
 
-  // rows i8 and i8 + 8: the queries, and their slots
-  float q[2][KL][4];
+  // rows i8 and i8 + 8: their slots, and the queries' operands, both terms, through shared memory (in registers they would
+  // be split again for every tile)
+  uint4* qop = reinterpret_cast<uint4*>(smem + C::kPart + C::kStat);  // [step][term][lane]
   int slot[2];
+  const float* src[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int r = r0 + i8 + 8 * e;
-    const bool live = i8 + 8 * e < rows;
-    const float* src = (const float*)p.q + b * p.qs[0] + (kh * G + r % G) * p.qs[1] + (int64_t)(r / G) * p.qs[2] + 4 * t4;
-#pragma unroll
-    for (int c = 0; c < KL; ++c) {
-      const float4 x = live ? *reinterpret_cast<const float4*>(src + 16 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-      q[e][c][0] = x.x; q[e][c][1] = x.y; q[e][c][2] = x.z; q[e][c][3] = x.w;
-    }
     slot[e] = row.first + r / G;
+    src[e] = i8 + 8 * e < rows ? (const float*)p.q + b * p.qs[0] + (kh * G + r % G) * p.qs[1] + (int64_t)(r / G) * p.qs[2] + 4 * t4
+                               : nullptr;
   }
+  for (int c = warp; c < KL; c += kWarps) {
+    float4 x[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) x[e] = src[e] ? *reinterpret_cast<const float4*>(src[e] + 16 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    qop[(4 * c + 0) * 32 + lane] = make_uint4(high(x[0].x), high(x[1].x), high(x[0].y), high(x[1].y));
+    qop[(4 * c + 1) * 32 + lane] = make_uint4(low(x[0].x), low(x[1].x), low(x[0].y), low(x[1].y));
+    qop[(4 * c + 2) * 32 + lane] = make_uint4(high(x[0].z), high(x[1].z), high(x[0].w), high(x[1].w));
+    qop[(4 * c + 3) * 32 + lane] = make_uint4(low(x[0].z), low(x[1].z), low(x[0].w), low(x[1].w));
+  }
+  __syncthreads();
 
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -137,16 +154,19 @@ __global__ void __launch_bounds__(kWarps * 32, F32Cfg<D>::kBlocks)
   }
   for (int tile = tile0; tile < tile1; ++tile) {
     float s[4] = {0.f, 0.f, 0.f, 0.f};         // (row i8, keys 2 t4 and + 1), (row i8 + 8, the same)
+    float s2[4] = {0.f, 0.f, 0.f, 0.f}, cross[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < KL; ++c)
 #pragma unroll
       for (int h = 0; h < 4; h += 2) {
-        const uint32_t ah[4] = {high(q[0][c][h]), high(q[1][c][h]), high(q[0][c][h + 1]), high(q[1][c][h + 1])};
-        const uint32_t al[4] = {low(q[0][c][h]), low(q[1][c][h]), low(q[0][c][h + 1]), low(q[1][c][h + 1])};
-        mma_tf32(s, al, high(kf[c][h]), high(kf[c][h + 1]));
-        mma_tf32(s, ah, low(kf[c][h]), low(kf[c][h + 1]));
-        mma_tf32(s, ah, high(kf[c][h]), high(kf[c][h + 1]));
+        const uint4 qh = qop[(4 * c + h) * 32 + lane], ql = qop[(4 * c + h + 1) * 32 + lane];
+        const uint32_t ah[4] = {qh.x, qh.y, qh.z, qh.w}, al[4] = {ql.x, ql.y, ql.z, ql.w};
+        mma_tf32(cross, al, high(kf[c][h]), high(kf[c][h + 1]));
+        mma_tf32(cross, ah, low(kf[c][h]), low(kf[c][h + 1]));
+        mma_tf32(h ? s2 : s, ah, high(kf[c][h]), high(kf[c][h + 1]));
       }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += s2[e] + cross[e];
     if (tile + 1 < tile1) load_k(tile + 1);
     int j, last;
     locate(tile, j, last);
@@ -197,9 +217,12 @@ __global__ void __launch_bounds__(kWarps * 32, F32Cfg<D>::kBlocks)
 #pragma unroll
       for (int h = 0; h < VW; ++h) {           // output column i8 is channel 8 VW c + VW i8 + h
         const float v0 = vf[0][c][h], v1 = vf[1][c][h];
-        mma_tf32(o[c * VW + h], al, high(v0), high(v1));
-        mma_tf32(o[c * VW + h], ah, low(v0), low(v1));
-        mma_tf32(o[c * VW + h], ah, high(v0), high(v1));
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_tf32(x, al, high(v0), high(v1));
+        mma_tf32(x, ah, low(v0), low(v1));
+        mma_tf32(x, ah, high(v0), high(v1));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[c * VW + h][e] += x[e];
       }
     if (tile + 1 < tile1) load_v(tile + 1);
   }
