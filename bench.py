@@ -608,13 +608,15 @@ def run_e2e(args, rank, world, dev):
     At N > 1 the ranks all-gather each step's logits.  Also reported,
     as the reference's perf runner does: time to first token (the prefill
     forward), time per output token and peak device memory; `--e2e-budget`
-    sets the cache budget (0.10 / 0.25 / 0.50 in the reference's sweep)."""
+    sets the cache budget (0.10 / 0.25 / 0.50 in the reference's sweep);
+    `--e2e-sample T` samples the tokens inside the same (replayed) steps."""
     import numpy as np
     import torch
     import torch.distributed as dist
     from transformers import LlamaConfig, LlamaForCausalLM
 
-    from stickykv_b200 import DecodeGraphs, WindowedCache, WindowedCacheConfig, install_score_hooks
+    from stickykv_b200 import (DecodeGraphs, WindowedCache, WindowedCacheConfig, install_score_hooks,
+                               sample_tokens)
 
     c = dict(E2E_8B if args.e2e_8b else E2E)
     if args.e2e_prompt:
@@ -659,11 +661,17 @@ def run_e2e(args, rank, world, dev):
         gathered = (torch.empty(world * rows, c["vocab"], dtype=torch.bfloat16, device=dev)
                     if world > 1 else None)
         tok = nxt.clone()
+        uniform = torch.empty(rows, dtype=torch.float32, device=dev)
 
         def decode_step(j=0):
             out = model(input_ids=tok, past_key_values=cache, use_cache=True, logits_to_keep=1)
             logits = gather_logits(out.logits[:, -1].contiguous(), gathered, world)
-            tok.copy_(logits[rank * rows:(rank + 1) * rows].argmax(-1, keepdim=True))
+            logits = logits[rank * rows:(rank + 1) * rows]
+            if args.e2e_sample:
+                uniform.uniform_()
+                tok.copy_(sample_tokens(logits, uniform, temperature=args.e2e_sample, top_k=50, top_p=0.95)[:, None])
+            else:
+                tok.copy_(logits.argmax(-1, keepdim=True))
 
         total = c["decode"] - 1
         # eager steps until the cache is in steady state (two evictions behind
@@ -713,8 +721,10 @@ def run_e2e(args, rank, world, dev):
         "value": total_rows * steps / (dec_ms * 1e-3), "n_gpus": world, "steps": steps,
         "ms_per_step": dec_ms / steps, "higher_is_better": True, "scaling": "strong",
         "dtype": "bf16 (int4 tier codes)", "data": "synthetic: random N(0,0.02) weights, uniform token ids",
-        "config": {"workload": f"{c['name']}: decoder with random weights, greedy decode through "
-                               "transformers with the windowed cache", "layers": c["layers"], "hidden": c["hidden"],
+        "config": {"workload": f"{c['name']}: decoder with random weights, "
+                               + (f"tokens sampled at temperature {args.e2e_sample:g}, top-k 50, top-p 0.95,"
+                                  if args.e2e_sample else "greedy decode")
+                               + " through transformers with the windowed cache", "layers": c["layers"], "hidden": c["hidden"],
                    "q_heads": c["heads"], "kv_heads": c["kv_heads"], "head_dim": c["head_dim"],
                    "global_batch": total_rows, "rows_per_gpu": rows, "prompt": c["prompt"],
                    "decode_steps": c["decode"],
@@ -1041,6 +1051,8 @@ def main():
                          "budget 0.25) instead of the Llama-3.2-1B one")
     ap.add_argument("--e2e-rows", type=int, default=0,
                     help="with --e2e: rows per GPU (default: the configuration's batch split over the GPUs)")
+    ap.add_argument("--e2e-sample", type=float, default=0.0, metavar="TEMPERATURE",
+                    help="model run: sample each token (top-k 50, top-p 0.95) instead of the largest logit")
     ap.add_argument("--e2e-eager", action="store_true",
                     help="decode the model run eagerly (no CUDA-graph replay of its steps)")
     ap.add_argument("--rows", type=int, default=0,

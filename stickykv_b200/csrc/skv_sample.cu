@@ -3,21 +3,31 @@
 //
 // In descending order with ties by index every cut is a threshold: the key of
 // the last kept token and how many of its equals, lowest indices first, stay.
-// No sort: a cluster holds a row in its blocks' shared memory and finds the
-// threshold with one histogram over evenly spaced values (below the maximum),
-// which names the bin that holds it, and a search among that bin's few tokens.
-// Rows whose bin holds too many (masses of equal logits) are searched bit by
-// bit over the whole row.
+// No sort.  A cluster holds a row in its blocks' shared memory; every 256
+// tokens' largest is kept beside them, and passes skip those below what they
+// look for.
+//   few of top-k   a value that k of those maxima reach bounds the cut; the
+//                  tokens from there on, little more than k, are listed;
+//   top-k, top-p   a histogram (counts, weights) over evenly spaced values
+//                  below the maximum names the bin that holds the cut; the
+//                  bin's tokens are listed, what lies above is summed exactly;
+// the cut is then found in the list, by comparing each with each or by 8 bits of
+// the keys a turn.  The sums prove that the list holds it; where it does not, or
+// equals overflow the list, the row is searched bit by bit.
 //
 // Weights and sums are 64-bit: a draw falls between two neighbours of 10^5
 // cumulative sums, and 32-bit sums would move a share of draws to a neighbour.
 // Sums are taken in a fixed order, or as whole numbers where the order is not
 // fixed, so equal calls give equal tokens.
 //
-// Bound: one row is latency (a handful of cluster barriers), many rows the
-// 64-bit exponentials of a top-p cut (about 16 operations a token at 64 a clock
-// and SM); HBM is read once.
+// Bound: one row is latency, three to six cluster barriers (32000 tokens: greedy
+// 2.9 us, top-k 50 12 us, with top-p 0.95 14 us); many rows the 64-bit
+// exponentials of a top-p cut, 13 operations a token at 59 a clock and SM, twice
+// (128 rows x 128256 bf16: greedy 12 us, 2.8 TB/s; temperature 43 us; top-p 0.9
+// 116 us).  HBM is read once.
 #include <float.h>
+
+#include <type_traits>
 
 #include "skv_common.cuh"
 
@@ -327,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       if (!(finite(blk_top[blk]) >= least)) continue;
       float v[8];
       load(blk, v);
-      f(blk, v);
+      f(v);
     }
   };
 
@@ -335,43 +345,41 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   {
     float mx = -INFINITY, mn = INFINITY;
     uint64_t best = 0;
-    constexpr int kAhead = 16 / sizeof(T) / 2;  // blocks whose loads are in flight together
-    P ahead[kAhead][kPacks];
-#pragma unroll 1
+    constexpr int kAhead = 8 / sizeof(T);  // blocks whose loads are in flight together
     for (int blk_a = warp; blk_a < n_blk; blk_a += kAhead * kWarps) {
+      P ahead[kAhead][kPacks];
 #pragma unroll
-     for (int a = 0; a < kAhead; ++a)
-      if (blk_a + a * kWarps < n_blk) fetch(blk_a + a * kWarps, ahead[a]);
+      for (int a = 0; a < kAhead; ++a)
+        if (blk_a + a * kWarps < n_blk) fetch(blk_a + a * kWarps, ahead[a]);
 #pragma unroll
-     for (int a = 0; a < kAhead; ++a) {
-      const int blk = blk_a + a * kWarps;
-      if (blk >= n_blk) break;
-      P(&v)[kPacks] = ahead[a];
+      for (int a = 0; a < kAhead; ++a) {
+        const int blk = blk_a + a * kWarps, i0 = (blk0 + blk) * kBlock + lane * 8;
+        if (blk >= n_blk) break;
+        P(&v)[kPacks] = ahead[a];
 #pragma unroll
-      for (int h = 0; h < kPacks; ++h) v[h].clean();
-      if (p.staged) {
-        uint4* s = reinterpret_cast<uint4*>(data + blk * kBlock + lane * 8);
+        for (int h = 0; h < kPacks; ++h) v[h].clean();
+        if (p.staged) {
+          uint4* s = reinterpret_cast<uint4*>(data + blk * kBlock + lane * 8);
 #pragma unroll
-        for (int h = 0; h < kPacks; ++h) s[h] = *reinterpret_cast<uint4*>(&v[h]);
+          for (int h = 0; h < kPacks; ++h) s[h] = *reinterpret_cast<uint4*>(&v[h]);
+        }
+        float hi = v[0].top(), lo = v[0].least();
+        if constexpr (kPacks > 1) hi = fmaxf(hi, v[1].top()), lo = fminf(lo, v[1].least());
+        mx = fmaxf(mx, hi);
+        if (i0 + 8 <= V) {
+          mn = fminf(mn, lo);
+        } else {  // without what fills up the last block
+          float f[8];
+#pragma unroll
+          for (int h = 0; h < kPacks; ++h) v[h].floats(f + h * P::N);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i0 + i < V) mn = fminf(mn, f[i]);
+        }
+        const uint32_t key = __reduce_max_sync(0xffffffffu, key_of(hi));
+        if (lane == 0) blk_top[blk] = value_of(key);
+        if (key > (uint32_t)(best >> 32)) best = (uint64_t)key << 32 | ~(uint32_t)(blk0 + blk);
       }
-      float hi = v[0].top(), lo = v[0].least();
-      if constexpr (kPacks > 1) hi = fmaxf(hi, v[1].top()), lo = fminf(lo, v[1].least());
-      mx = fmaxf(mx, hi);
-      const int i0 = (blk0 + blk) * kBlock + lane * 8;
-      if (i0 + 8 <= V) {
-        mn = fminf(mn, lo);
-      } else {  // without what fills up the last block
-        float f[8];
-#pragma unroll
-        for (int h = 0; h < kPacks; ++h) v[h].floats(f + h * P::N);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i0 + i < V) mn = fminf(mn, f[i]);
-      }
-      const uint32_t key = __reduce_max_sync(0xffffffffu, key_of(hi));
-      if (lane == 0) blk_top[blk] = value_of(key);
-      if (key > (uint32_t)(best >> 32)) best = (uint64_t)key << 32 | ~(uint32_t)(blk0 + blk);
-     }
     }
     const uint32_t lane_min = __reduce_min_sync(0xffffffffu, key_of(mx)), low = __reduce_min_sync(0xffffffffu, key_of(mn));
     if (lane == 0) {
@@ -449,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   auto count_from = [&](uint32_t t) {
     uint32_t n = 0;
     const float least = value_of(t);
-    each8(least, [&](int, const float (&v)[8]) {
+    each8(least, [&](const float (&v)[8]) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) n += v[i] >= least;
     });
@@ -461,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   auto mass_from = [&](uint32_t t) {
     double s = 0;
     const float least = value_of(max(max(t, tau + 1), low_key));
-    each8(least, [&](int, const float (&v)[8]) {
+    each8(least, [&](const float (&v)[8]) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const double e = weight(v[i]);
@@ -489,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   auto lowest = [&]() -> float {           // the smallest logit above -inf
     if (least_key == kNone) {
       float mn = INFINITY;
-      each8(-FLT_MAX, [&](int, const float (&v)[8]) {
+      each8(-FLT_MAX, [&](const float (&v)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (v[i] > -INFINITY) mn = fminf(mn, v[i]);
@@ -541,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
     uint32_t lo_k = 0xffffffffu, hi_k = 0;
     for (int i = tid; i < 4 * 3 * 256; i += kThreads) digits[0][0][i] = 0;
     low = fmaxf(low, tau ? value_of(tau) : -FLT_MAX);
-    each8(least, [&](int, const float (&v)[8]) {
+    each8(least, [&](const float (&v)[8]) {
       also(v);
       uint32_t n = 0;
 #pragma unroll
@@ -738,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
     if (low == -INFINITY) low = lowest();
     spread(m - low);
     if (tid == 0) sh.last = -1;
-    each8(low, [&](int, const float (&v)[8]) {  // the last bin holds all that is further down: not counted
+    each8(low, [&](const float (&v)[8]) {  // the last bin holds all that is further down: not counted
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float d = depth(v[i]);
@@ -848,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       const float fall = per_unit > 0.f ? 1.f / (per_unit * temp) : 0.f;  // of the weight's logarithm over a bin
       if (tid == 0) sh.last = -1;
       const float kept_from = value_of(max(low_key, tau + 1));
-      each8(kept_from, [&](int, const float (&v)[8]) {
+      each8(kept_from, [&](const float (&v)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float d = depth(v[i]), t = place(d), off = (t - 8388608.f - d) * fall;
@@ -1072,10 +1080,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
 template <typename T>
 int launch(SampleParams p, int batch, cudaStream_t stream) {
   static std::atomic<uint32_t> done{0};
-  constexpr int kMost = 160 * 1024;  // of shared memory, beside the histogram and the list
+  constexpr int kMost = 160 * 1024;  // bytes of a row's share in shared memory, beside 36 KB of histogram and list
   const int blocks = ceil_div(p.V, kBlock);
-  // a cluster as large as keeps every block's warps busy and all rows resident
-  // at once, and at least as large as holds the row
+  // a cluster at least as large as holds the row, and as large as keeps every
+  // warp busy with all rows resident (a block an SM, of 114 registers a thread:
+  // 33 rows on clusters of 8, two rounds, took twice as long as on 4)
   int c = 1;
   auto bytes = [&](int n) {
     const size_t per = ceil_div(blocks, n);

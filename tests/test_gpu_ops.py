@@ -282,6 +282,57 @@ def test_window_strides(dt, T):
     assert skv.sink_window_attention(q, k, v, window=50, sinks=3, out=place) is place and torch.equal(place, want)
 
 
+@pytest.mark.parametrize("dt, D", [("f32", 32), ("f16", 64), ("bf16", 128), ("f16", 32)])
+@pytest.mark.parametrize("Hq, Hkv", [(128, 1), (256, 1), (260, 2), (100, 1)])
+def test_window_many_heads_to_a_kv_head(dt, D, Hq, Hkv):
+    """Groups of 100 to 256 query heads: as large as a tile, larger, and of no
+    divisor in common with it."""
+    for T, S in ((1, 200), (5, 200), (70, 70)):
+        q, k, v = qkv(2, T, S, Hq, Hkv, D, dt, T)
+        check_window(q, k, v, 60, 3)
+
+
+@pytest.mark.parametrize("dt, D", [("bf16", 64), ("f16", 128), ("f32", 64)])
+@pytest.mark.parametrize("T", [1, 200, 900])
+def test_window_lengths_around_tiles(dt, D, T):
+    """First tokens and windows that end on, before and behind the borders of
+    8- and 128-key tiles."""
+    q, k, v = qkv(1, T, 900, 4, 1, D, dt, T)
+    for sinks in (0, 1, 7, 8, 9, 127, 128, 129, 300):
+        for window in (1, 2, 63, 64, 65, 127, 128, 129, 500):
+            check_window(q, k, v, window, sinks)
+
+
+def test_window_repeated_calls_are_checked_again():
+    """Calls alike in shapes and settings: another input that asks for
+    gradients, is misaligned or on the host is refused or copied all the same."""
+    q, k, v = qkv(2, 1, 64, 4, 2, 64, "f16", 1)
+    want = [skv.sink_window_attention(q, k, v, window=9) for _ in range(3)][-1]
+    base = torch.empty(k.numel() + 1, dtype=k.dtype, device="cuda")
+    odd = base[1:].view(k.shape)
+    odd.copy_(k)
+    assert odd.stride() == k.stride() and odd.data_ptr() % 16
+    assert torch.equal(skv.sink_window_attention(q, odd, v, window=9), want)
+    with pytest.raises(NotImplementedError):
+        skv.sink_window_attention(q.clone().requires_grad_(), k, v, window=9)
+    with pytest.raises(ValueError):
+        skv.sink_window_attention(q, k.cpu(), v, window=9)
+    inv, _ = skv.rotary_frequencies(64, device="cuda")
+    pos = torch.arange(1, device="cuda")
+    a = [skv.apply_rotary(q, k[:, :, :1], pos, inv) for _ in range(3)]
+    assert all(torch.equal(x, y) for x, y in zip(a[0], a[2]))
+    with pytest.raises(NotImplementedError):
+        skv.apply_rotary(q.clone().requires_grad_(), k[:, :, :1], pos, inv)
+    x, u = torch.randn(2, 99, device="cuda"), torch.rand(2, device="cuda")
+    b = [skv.sample_tokens(x, u, top_k=5) for _ in range(3)]
+    assert torch.equal(b[0], b[2])
+    check_sample(x, u, top_k=6)
+    with pytest.raises(NotImplementedError):
+        skv.sample_tokens(x.clone().requires_grad_(), u, top_k=5)
+    with pytest.raises(ValueError):
+        skv.sample_tokens(x, u.cpu(), top_k=5)
+
+
 def test_window_past_32_bit_offsets():
     """A cache of over 2^31 elements, most of it never written; decode and a
     chunk at its far end and, with sinks, at its beginning."""
@@ -395,6 +446,47 @@ def test_sample_ties_and_masks(dt):
                    dict(temperature=0.7, top_p=0.25, top_k=2)):
             got = check_sample(x, u, **kw)
             assert got[3] == -1 and got[4] == -1 and got[2] == 1234 and got[8] in (17, 2900)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_sample_cuts_among_equals(dt):
+    """Cuts that fall inside runs of equal logits, at the head of the order and
+    far down, with lists that hold the run and runs that no list holds."""
+    V = 20000
+    g = gen(31)
+    u = torch.rand(6, generator=g, device="cuda")
+    x = normal((6, V), torch.float32, g)
+    x[0] = x[0].round()                       # thousands of equals each
+    x[1] = (x[1] * 4).round() / 4
+    x[2, 1000:1300] = 5.0                     # a run of 300 above the rest
+    x[3, ::7] = 6.0                           # a run of 2858 above the rest
+    x[4, 1::2] = -math.inf
+    x[5] = x[5].clamp(max=0.5)
+    x = x.to(DT[dt])
+    for kw in (dict(top_k=40), dict(top_k=299), dict(top_k=301), dict(top_k=2500), dict(top_k=3000), dict(top_k=9999), dict(top_k=15000),
+               dict(top_p=0.1), dict(top_p=0.5), dict(top_p=0.97), dict(top_k=150, top_p=0.5), dict(top_k=2900, top_p=0.3),
+               dict(top_k=12000, top_p=0.8, temperature=3.0), dict(temperature=0.05, top_p=0.9), dict(top_p=0.999999)):
+        check_sample(x, u, **kw)
+
+
+def test_sample_extreme_scales():
+    """Logits and temperatures near the ends of their types."""
+    g = gen(41)
+    V = 3000
+    u = torch.rand(4, generator=g, device="cuda")
+    for scale in (1e-30, 1e-6, 1e4, 1e30, 3e38):
+        x = (torch.rand(4, V, generator=g, device="cuda") * 2 - 1) * scale
+        for temperature in (1e-38, 1e-3, 1.0, 1e3, 1e38):
+            for kw in (dict(), dict(top_k=30, top_p=0.9), dict(top_p=0.7), dict(top_k=2000, min_p=0.5)):
+                check_sample(x, u, temperature=temperature, **kw)
+
+
+def test_sample_random_numbers_out_of_range_stay_in_the_vocabulary():
+    x = normal((5, 1000), torch.float32, gen(5))
+    u = torch.tensor([1.0, 2.0, -1.0, math.nan, math.inf], device="cuda")
+    for kw in (dict(), dict(top_k=7), dict(top_p=0.9)):
+        got = skv.sample_tokens(x, u, **kw)
+        assert ((got >= 0) & (got < 1000)).all()
 
 
 def test_sample_rows_apart_and_odd_bases():
