@@ -46,12 +46,14 @@ template <int D> struct ManyCfg {
 };
 
 struct ManyMaps {
-  CUtensorMap q, k, v, k8, v8;
+  CUtensorMap q, k, v;         // boxes of a tile's rows
+  CUtensorMap k8, v8;          // of 8 rows: first tokens
+  CUtensorMap k_rest, v_rest;  // of what the usual first tokens leave of a tile
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
-    window_many_kernel(const __grid_constant__ WindowParams p, const __grid_constant__ ManyMaps maps) {
+    window_many_kernel(const __grid_constant__ WindowParams p, const __grid_constant__ ManyMaps maps, int firsts) {
   using C = ManyCfg<D>;
   constexpr bool kBF = !std::is_same<T, __half>::value;
   constexpr uint32_t kIdS = idesc(kBF, kRows, kRows, false), kIdO = idesc(kBF, kRows, D, true);
@@ -109,11 +111,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (v0 + kRows <= A8 || v0 >= A8) {
       const int slot = v0 >= A8 ? w0 + v0 - A8 : a0 + v0;
       for (int h = 0; h < D / 64; ++h) tma4(dst + h * C::kHalf, map, bar, 64 * h, slot, ch, cb);
-    } else {  // both runs in one tile: 8 rows at a time
-      for (int r = 0; r < kRows; r += 8) {
-        const int slot = v0 + r >= A8 ? w0 + v0 + r - A8 : a0 + v0 + r;
+    } else {  // both runs in one tile: first tokens 8 rows at a time; the window's in one box where there are as many as usual
+      const int cut = A8 - v0;
+      const bool usual = A8 == firsts;
+      for (int r = 0; r < (usual ? cut : kRows); r += 8) {
+        const int slot = r < cut ? a0 + v0 + r : w0 + r - cut;
         for (int h = 0; h < D / 64; ++h) tma4(dst + h * C::kHalf + r * 128, map8, bar, 64 * h, slot, ch, cb);
       }
+      if (usual)
+        for (int h = 0; h < D / 64; ++h)
+          tma4(dst + h * C::kHalf + cut * 128, val ? &maps.v_rest : &maps.k_rest, bar, 64 * h, w0, ch, cb);
     }
   };
   if (warp == 9 && lane == 0) {
@@ -128,14 +135,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     fence_proxy();
-    if (n > 0) {  // the queries and the first tile are on their way before the block has met
+    if (n > 0) {  // the queries are on their way before the block has met
       const int nq = i0 + TQ < p.T ? 2 : 1;
       bar_expect(bQ, nq * G * TQ * D * 2);
       for (int t = 0; t < nq; ++t)
         for (int h = 0; h < D / 64; ++h)
           tma5(sQ + t * C::kTile + h * C::kHalf, &maps.q, bQ, 64 * h, 0, i0 + t * TQ, kh, p.qs[0] ? b : 0);
       load_kv(0);
-      load_kv(1);
     }
   }
   fence_before();
@@ -150,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n" ::);
    if (warp == 9) {
     if (lane == 0) {
-      for (int x = 2; x < 2 * n; ++x) {
+      for (int x = 1; x < 2 * n; ++x) {
         const int s = x % C::kStages, use = x / C::kStages;
         if (use > 0 && !bar_wait(bFree + 8 * s, (use - 1) & 1)) break;
         load_kv(x);
@@ -394,17 +400,19 @@ int launch_many(const WindowParams& p, cudaStream_t stream) {
     const uint32_t box[5] = {64, (uint32_t)G, (uint32_t)TQ, 1, 1};
     if (!encode(&maps.q, kBF, 5, p.q, dims, st, box)) return SKV_ERR_CUDA;
   }
-  CUtensorMap* const out[4] = {&maps.k, &maps.v, &maps.k8, &maps.v8};
-  for (int i = 0; i < 4; ++i) {
+  // the usual count of first tokens, rounded up as the kernel does, and what it leaves of the tile that both runs share
+  const int firsts = (int)align_up(p.sinks, 8), rest = kRows - firsts % kRows;
+  CUtensorMap* const out[6] = {&maps.k, &maps.v, &maps.k8, &maps.v8, &maps.k_rest, &maps.v_rest};
+  for (int i = 0; i < 6; ++i) {
     const int64_t* s = i & 1 ? p.vs : p.ks;
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)p.S, count(s[1], p.Hkv), count(s[0], p.B)};
     const uint64_t st[3] = {step(s[2], p.S), step(s[1], p.Hkv), step(s[0], p.B)};
-    const uint32_t box[4] = {64, i < 2 ? 128u : 8u, 1, 1};
+    const uint32_t box[4] = {64, i < 2 ? (uint32_t)kRows : i < 4 ? 8u : (uint32_t)rest, 1, 1};
     if (!encode(out[i], kBF, 4, i & 1 ? p.v : p.k, dims, st, box)) return SKV_ERR_CUDA;
   }
   max_smem_once(done, window_many_kernel<T, D>, (int)C::kSmem);
   const dim3 grid((unsigned)ceil_div64(p.T, 2 * TQ), p.Hkv, p.B);
-  window_many_kernel<T, D><<<grid, kThreads, C::kSmem, stream>>>(p, maps);
+  window_many_kernel<T, D><<<grid, kThreads, C::kSmem, stream>>>(p, maps, firsts);
   SKV_CHECK_LAUNCH();
   return SKV_OK;
 }
