@@ -14,6 +14,25 @@ bool window_many_supported(const WindowParams& p);
 int window_many(const WindowParams& p, int dtype, cudaStream_t stream);
 namespace {
 
+// Which kernel takes an fp16 or bf16 call: the one that is done first by these
+// estimates, in ns.  Few rows: blocks of 16 rows that read every key they see,
+// 40 ps a key and block (head_dim 64; 80 at 128) over the whole GPU.  Many rows:
+// rounds of a block an SM, 5 us and 1.25 us a 128-key tile (1.65 where the block
+// has a second tile of rows).  Measured, few/many, 32/8 heads of 64 over 4000
+// keys: 1 row, 4 tokens 10/39 us, 64 tokens 28/56, 128 tokens 46/56; 16 rows, 4
+// tokens 34/41, 8 tokens 54/41, 128 tokens 629/113.
+bool many_is_faster(const WindowParams& p) {
+  const int64_t G = p.Hq / p.Hkv, tile = 128 / G;
+  auto keys = [&](int64_t tokens) {  // that so many neighbouring tokens see
+    return std::min<int64_t>(p.S, (int64_t)p.sinks + p.window + std::min<int64_t>(tokens, p.T));
+  };
+  const int64_t groups = ceil_div64(p.T * G, 16) * p.Hkv * p.B;
+  const int64_t rounds = ceil_div64(ceil_div64(p.T, 2 * tile) * p.Hkv * p.B, 148);
+  const double few = 4000.0 + 0.040 * (p.D / 64.0) * groups * keys(16 / G);
+  const double many = rounds * (5000.0 + ceil_div64(keys(2 * tile), 128) * (p.T > tile ? 1650.0 : 1250.0));
+  return many < few;
+}
+
 int check_window(const skv_window_args* a) {
   if (!a) return SKV_ERR_INVALID_ARG;
   if (a->batch <= 0 || a->q_tokens <= 0 || a->k_slots <= 0 || a->num_q_heads <= 0 || a->num_kv_heads <= 0)
@@ -24,7 +43,7 @@ int check_window(const skv_window_args* a) {
   const int es = a->dtype == SKV_F32 ? 4 : (a->dtype == SKV_F16 || a->dtype == SKV_BF16) ? 2 : 0;
   if (!es) return SKV_ERR_UNSUPPORTED;
   // heads and rows index grid dimensions; slots and queries 31-bit sums
-  if (a->batch > 65535 || a->num_q_heads > 65535 || a->k_slots > (1 << 30) || a->q_tokens > (1 << 30))
+  if (a->batch > 65535 || a->num_q_heads > 65535 || a->k_slots > (1 << 29) || a->q_tokens > (1 << 29))
     return SKV_ERR_UNSUPPORTED;
   const void* ptrs[4] = {a->q, a->k, a->v, a->out};
   for (const void* x : ptrs)
@@ -62,6 +81,6 @@ extern "C" int skv_window_attention(const skv_window_args* a, void* stream) {
   p.scaling = a->scaling;
   const cudaStream_t s = (cudaStream_t)stream;
   if (a->dtype == SKV_F32) return window_f32(p, s);
-  if ((int64_t)p.T * (p.Hq / p.Hkv) > 64 && window_many_supported(p)) return window_many(p, a->dtype, s);
+  if (window_many_supported(p) && many_is_faster(p)) return window_many(p, a->dtype, s);
   return window_few(p, a->dtype, s);
 }

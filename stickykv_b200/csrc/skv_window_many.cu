@@ -153,82 +153,82 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // 168 registers a thread at launch, three warpgroups: 2 x 208 + 80 of the 504 they share
   if (warp >= 8) {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n" ::);
-   if (warp == 9) {
-    if (lane == 0) {
-      for (int x = 1; x < 2 * n; ++x) {
-        const int s = x % C::kStages, use = x / C::kStages;
-        if (use > 0 && !bar_wait(bFree + 8 * s, (use - 1) & 1)) break;
-        load_kv(x);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n" ::);
+    if (warp == 9) {
+      if (lane == 0) {
+        for (int x = 1; x < 2 * n; ++x) {
+          const int s = x % C::kStages, use = x / C::kStages;
+          if (use > 0 && !bar_wait(bFree + 8 * s, (use - 1) & 1)) break;
+          load_kv(x);
+        }
       }
-    }
-   } else if (warp == 8) {
-    if (n > 0) {
-      auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (!lost && !bar_wait(bar, parity)) lost = true;
-        lost = __any_sync(0xffffffffu, lost);
-        fence_after();
-      };
-      auto full = [&](int x) { wait(bFull + 8 * (x % C::kStages), (x / C::kStages) & 1); };
-      auto issue_s = [&](int t, int j) {
-        const uint64_t q = desc_k(sQ + t * C::kTile), k = desc_k(sR + (2 * j % C::kStages) * C::kTile);
+    } else if (warp == 8) {
+      if (n > 0) {
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+          if (!lost && !bar_wait(bar, parity)) lost = true;
+          lost = __any_sync(0xffffffffu, lost);
+          fence_after();
+        };
+        auto full = [&](int x) { wait(bFull + 8 * (x % C::kStages), (x / C::kStages) & 1); };
+        auto issue_s = [&](int t, int j) {
+          const uint64_t q = desc_k(sQ + t * C::kTile), k = desc_k(sR + (2 * j % C::kStages) * C::kTile);
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) {
-          const uint32_t off = ((e >> 2) * C::kHalf + (e & 3) * 32) >> 4;
-          mma_ss(tmem + t * kRows, q + off, k + off, kIdS, e > 0);
-        }
-        commit(bS + 8 * t);
-      };
-      // P's first three quarters are there before the last: the product begins with them
-      auto issue_o = [&](int t, int j) {
-        const uint64_t v = desc_mn(sR + ((2 * j + 1) % C::kStages) * C::kTile, C::kHalf);
-        const uint32_t first = j > lo[t], par = (j - lo[t]) & 1;
-        wait(bP + 8 * t, par);
-        full(2 * j + 1);
+          for (int e = 0; e < D / 16; ++e) {
+            const uint32_t off = ((e >> 2) * C::kHalf + (e & 3) * 32) >> 4;
+            mma_ss(tmem + t * kRows, q + off, k + off, kIdS, e > 0);
+          }
+          commit(bS + 8 * t);
+        };
+        // P's first three quarters are there before the last: the product begins with them
+        auto issue_o = [&](int t, int j) {
+          const uint64_t v = desc_mn(sR + ((2 * j + 1) % C::kStages) * C::kTile, C::kHalf);
+          const uint32_t first = j > lo[t], par = (j - lo[t]) & 1;
+          wait(bP + 8 * t, par);
+          full(2 * j + 1);
 #pragma unroll
-        for (int e = 0; e < kRows / 16; ++e) {
-          if (e == 6) wait(bP2 + 8 * t, par);
-          mma_ts(tmem + C::kO + t * D, tmem + C::kP + t * C::kPStep + 8 * e, v + (e * 16 * 128 >> 4), kIdO, e > 0 ? 1u : first);
-        }
-        commit(bO + 8 * t);
-      };
-      auto next_s = [&](int t, int j) {
-        if (j + 1 >= lo[t] && j + 1 < hi[t]) {
-          if (C::kApart && j >= lo[t]) wait(bL + 8 * t, (j - lo[t]) & 1);  // this S has been read
-          full(2 * j + 2);
-          issue_s(t, j + 1);
-        }
-      };
-      wait(bQ, 0);
-      full(0);
+          for (int e = 0; e < kRows / 16; ++e) {
+            if (e == 6) wait(bP2 + 8 * t, par);
+            mma_ts(tmem + C::kO + t * D, tmem + C::kP + t * C::kPStep + 8 * e, v + (e * 16 * 128 >> 4), kIdO, e > 0 ? 1u : first);
+          }
+          commit(bO + 8 * t);
+        };
+        auto next_s = [&](int t, int j) {
+          if (j + 1 >= lo[t] && j + 1 < hi[t]) {
+            if (C::kApart && j >= lo[t]) wait(bL + 8 * t, (j - lo[t]) & 1);  // this S has been read
+            full(2 * j + 2);
+            issue_s(t, j + 1);
+          }
+        };
+        wait(bQ, 0);
+        full(0);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (lo[t] == 0 && hi[t] > 0) issue_s(t, 0);
-      commit(bFree);
-      for (int j = 0; j < n; ++j) {
-        if (C::kApart) {
+        for (int t = 0; t < 2; ++t)
+          if (lo[t] == 0 && hi[t] > 0) issue_s(t, 0);
+        commit(bFree);
+        for (int j = 0; j < n; ++j) {
+          if (C::kApart) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) next_s(t, j);
-          if (j + 1 < n) {
+            for (int t = 0; t < 2; ++t) next_s(t, j);
+            if (j + 1 < n) {
+              full(2 * j + 2);
+              commit(bFree + 8 * ((2 * j + 2) % C::kStages));
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= lo[t] && j < hi[t]) issue_o(t, j);
+            if (!C::kApart) next_s(t, j);
+          }
+          full(2 * j + 1);
+          commit(bFree + 8 * ((2 * j + 1) % C::kStages));
+          if (!C::kApart && j + 1 < n) {
             full(2 * j + 2);
             commit(bFree + 8 * ((2 * j + 2) % C::kStages));
           }
         }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (j >= lo[t] && j < hi[t]) issue_o(t, j);
-          if (!C::kApart) next_s(t, j);
-        }
-        full(2 * j + 1);
-        commit(bFree + 8 * ((2 * j + 1) % C::kStages));
-        if (!C::kApart && j + 1 < n) {
-          full(2 * j + 2);
-          commit(bFree + 8 * ((2 * j + 2) % C::kStages));
-        }
       }
+      __syncwarp();
     }
-    __syncwarp();
-   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n" ::);
     const int t = warp >> 2, rl = threadIdx.x & 127;
@@ -371,6 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // a key that is not finite reaches the rows that do not see it as 0 * inf:
     // rows that come out not finite are done again key by key
+    __syncwarp();  // behind the stores above
     uint32_t again = __ballot_sync(0xffffffffu, bad && real);
     while (again) {
       const int who = __ffs(again) - 1;

@@ -213,24 +213,46 @@ def test_window(B, T, S, Hq, Hkv, window, sinks, dt, D):
     check_window(q, k, v, window, sinks)
 
 
+@pytest.mark.parametrize("dt, D", [("f16", 64), ("bf16", 64), ("f16", 128), ("bf16", 128)])
+@pytest.mark.parametrize("T, S, Hq, Hkv", [(64, 64, 4, 4), (100, 100, 8, 2), (127, 127, 4, 1), (128, 128, 4, 2), (129, 257, 8, 2),
+                                           (260, 260, 3, 3), (300, 1111, 8, 2), (90, 90, 100, 1), (33, 33, 128, 1)])
+def test_window_batches_of_prompts(T, S, Hq, Hkv, dt, D):
+    """As many blocks of two row tiles as fill the GPU once."""
+    tokens = 2 * (128 // (Hq // Hkv))
+    B = -(-148 // (-(-T // tokens) * Hkv))
+    q, k, v = qkv(B, T, S, Hq, Hkv, D, dt, T + Hq)
+    for window, sinks in ((1, 0), (17, 3), (60, 5), (100, 8), (128, 130), (None, 0)):
+        check_window(q, k, v, window, sinks)
+    # a cache longer than its use, tokens before heads, one row or head for all
+    room = torch.full((B, Hkv, S + 23, D), math.nan, dtype=DT[dt], device="cuda")
+    room[:, :, 7:7 + S] = k
+    want = skv.sink_window_attention(q, k, v, window=128, sinks=9)
+    assert torch.equal(want, skv.sink_window_attention(q.contiguous(), room[:, :, 7:7 + S], v.transpose(1, 2).contiguous().transpose(1, 2),
+                                                       window=128, sinks=9))
+    one_row, one_head = k[:1].expand_as(k), v[:, :1].expand_as(v)
+    assert torch.equal(skv.sink_window_attention(q, one_row, one_head, window=128, sinks=9),
+                       skv.sink_window_attention(q, one_row.contiguous(), one_head.contiguous(), window=128, sinks=9))
+
+
 @pytest.mark.parametrize("dt, D", [("f32", 32), ("f16", 64), ("bf16", 64), ("bf16", 128)])
 @pytest.mark.parametrize("T", [1, 3, 150, 400])
-def test_window_rows_of_unlike_length(dt, D, T):
+@pytest.mark.parametrize("copies", [1, 9])
+def test_window_rows_of_unlike_length(dt, D, T, copies):
     """Left and right padding, rows of no token and of one, queries before and
     behind their row; what lies in the padding is NaN or infinite and reaches no
     output, and a query that sees nothing gives zeros."""
-    B, S = 6, 400
+    B, S = 6 * copies, 400
     q, k, v = qkv(B, T, S, 8, 2, D, dt, T)
-    starts = torch.tensor([0, 399, 37, 400, 128, -5], dtype=torch.int32, device="cuda")
-    ends = torch.tensor([400, 400, 300, 400, 129, 1000], dtype=torch.int32, device="cuda")
-    for i, bad in enumerate((math.nan, math.inf, -math.inf, math.nan, math.inf, math.nan)):
+    starts = torch.tensor([0, 399, 37, 400, 128, -5], dtype=torch.int32, device="cuda").repeat(copies)
+    ends = torch.tensor([400, 400, 300, 400, 129, 1000], dtype=torch.int32, device="cuda").repeat(copies)
+    first = torch.tensor([0, 398, 30, 0, 127, 200], dtype=torch.int32, device="cuda").repeat(copies)
+    for i, bad in enumerate((math.nan, math.inf, -math.inf, math.nan, math.inf, math.nan) * copies):
         dead = torch.ones(S, dtype=torch.bool, device="cuda")
         dead[max(0, int(starts[i])):int(ends[i])] = False
         k[i, :, dead] = bad
         v[i, :, dead] = bad
     for window, sinks in ((20, 4), (None, 0), (129, 140), (1, 1)):
-        for slots in (None, torch.full((B,), S - T, dtype=torch.int32, device="cuda"),
-                      torch.tensor([0, 398, 30, 0, 127, 200], dtype=torch.int32, device="cuda")):
+        for slots in (None, torch.full((B,), S - T, dtype=torch.int32, device="cuda"), first):
             got = check_window(q, k, v, window, sinks, starts=starts, ends=ends, query_slots=slots)
             assert not got[3].any()
     got = check_window(q, k, v, 20, 4, ends=torch.zeros(B, dtype=torch.int32, device="cuda"))
@@ -238,11 +260,12 @@ def test_window_rows_of_unlike_length(dt, D, T):
 
 
 @pytest.mark.parametrize("dt, D, T", [("f32", 32, 200), ("f16", 64, 200), ("bf16", 128, 333), ("f16", 128, 1), ("bf16", 64, 3)])
-def test_window_unseen_tokens_may_hold_anything(dt, D, T):
+@pytest.mark.parametrize("rows", [1, 40])
+def test_window_unseen_tokens_may_hold_anything(dt, D, T, rows):
     """Live tokens that some queries see and others do not: one that is not
     finite reaches exactly the queries that see it."""
     S, window, sinks = 333, 40, 2
-    q, k, v = qkv(1, T, S, 4, 2, D, dt, 3)
+    q, k, v = qkv(rows, T, S, 4, 2, D, dt, 3)
     at = [S - T, S - 60, S - 1] if T > 60 else [S - 60, S - 50]
     clean = v.clone()
     for n, j in enumerate(at):
@@ -258,11 +281,11 @@ def test_window_unseen_tokens_may_hold_anything(dt, D, T):
 
 
 @pytest.mark.parametrize("dt", DT)
-@pytest.mark.parametrize("T", [1, 40])
-def test_window_strides(dt, T):
+@pytest.mark.parametrize("B, T", [(2, 1), (2, 40), (60, 150)])
+def test_window_strides(dt, B, T):
     """Caches longer than their use, heads and tokens in any order, bases and
     rows that are not 16-byte aligned, heads shared by expansion."""
-    B, S, Hq, Hkv, D = 2, 200, 6, 2, 64
+    S, Hq, Hkv, D = 200, 6, 2, 64
     q, k, v = qkv(B, T, S, Hq, Hkv, D, dt, 4)
     want = check_window(q, k, v, 50, 3)
     room = torch.full((B, Hkv, S + 57, D), math.nan, dtype=DT[dt], device="cuda")
@@ -293,11 +316,11 @@ def test_window_many_heads_to_a_kv_head(dt, D, Hq, Hkv):
 
 
 @pytest.mark.parametrize("dt, D", [("bf16", 64), ("f16", 128), ("f32", 64)])
-@pytest.mark.parametrize("T", [1, 200, 900])
-def test_window_lengths_around_tiles(dt, D, T):
+@pytest.mark.parametrize("B, T", [(1, 1), (1, 200), (1, 900), (12, 900)])
+def test_window_lengths_around_tiles(dt, D, B, T):
     """First tokens and windows that end on, before and behind the borders of
     8- and 128-key tiles."""
-    q, k, v = qkv(1, T, 900, 4, 1, D, dt, T)
+    q, k, v = qkv(B, T, 900, 4, 1, D, dt, T)
     for sinks in (0, 1, 7, 8, 9, 127, 128, 129, 300):
         for window in (1, 2, 63, 64, 65, 127, 128, 129, 500):
             check_window(q, k, v, window, sinks)
@@ -343,10 +366,11 @@ def test_window_past_32_bit_offsets():
         x[:, :, -700:] = normal((B, Hkv, 700, D), torch.float16, g)
         x[:, :, :4] = normal((B, Hkv, 4, D), torch.float16, g)
     near = [torch.cat((x[:, :, :4], x[:, :, -700:]), 2) for x in (k, v)]
-    for T in (1, 200):
-        q = normal((B, 4, T, D), torch.float16, g)
-        got = skv.sink_window_attention(q, k, v, window=400, sinks=4)
-        ref = window_ref(q, *near, 400, 4)
+    for T in (1, 200, 690):
+        q = normal((B, 64, T, D), torch.float16, g)
+        window = min(400, 700 - T)
+        got = skv.sink_window_attention(q, k, v, window=window, sinks=4)
+        ref = window_ref(q, *near, window, 4)
         within(got, ref[0], window_tol(q, ref))
     del k, v
     torch.cuda.empty_cache()
@@ -355,8 +379,8 @@ def test_window_past_32_bit_offsets():
 def test_window_large_scores_and_lowest_values():
     """Scores far apart, and keys of the type's lowest value."""
     for dt in ("f16", "bf16", "f32"):
-        for T in (1, 200):
-            q, k, v = qkv(1, T, 300, 4, 2, 64, dt, 6)
+        for B, T in ((1, 1), (1, 200), (30, 200)):
+            q, k, v = qkv(B, T, 300, 4, 2, 64, dt, 6)
             check_window(q, k, v, 70, 4, scaling=4.0)
             check_window(q, k, v, 70, 4, scaling=-0.5)
             check_window(q, k, v, 70, 4, scaling=0.0)
