@@ -87,11 +87,21 @@ template <typename T, int V, bool kInter>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
   using RT = typename Raw<sizeof(T) * V>::type;
   __shared__ __align__(16) float2 turns[kChunks * V];  // cosine, sine
-  const int64_t first = blockIdx.x * (int64_t)kChunks, rows = (int64_t)p.B * p.T;
-  const int64_t id = first + threadIdx.x % kChunks, row = id / p.chunks;
-  const int c = (int)(id % p.chunks);
-  const bool live = row < rows;
-  const int b = live ? (int)(row / p.T) : 0, t = live ? (int)(row % p.T) : 0;
+  __shared__ double where[kChunks];                    // position / 2 pi
+  __shared__ int batch[kChunks], token[kChunks], chunk[kChunks];  // batch < 0: behind the last row
+  if (threadIdx.x < kChunks) {                         // the divisions, once a chunk
+    const uint64_t id = blockIdx.x * (uint64_t)kChunks + threadIdx.x;
+    const uint32_t row = id >> 32 ? (uint32_t)(id / p.chunks) : (uint32_t)id / p.chunks;
+    const bool live = row < (uint32_t)p.B * (uint32_t)p.T;
+    const int b = live ? (int)(row / (uint32_t)p.T) : -1, t = live ? (int)(row % (uint32_t)p.T) : 0;
+    batch[threadIdx.x] = b;
+    token[threadIdx.x] = t;
+    chunk[threadIdx.x] = (int)(id - (uint64_t)row * p.chunks);
+    where[threadIdx.x] = live ? (double)p.pos[b * p.ps_b + t * p.ps_t] * 0.15915494309189533577 : 0.0;
+  }
+  __syncthreads();
+  const int mine = threadIdx.x % kChunks;
+  const int b = batch[mine], t = token[mine], c = chunk[mine];
   const bool rot = c < p.rot_chunks;
   int c0, c1;              // first channels of the two vectors
   if (rot) {
@@ -103,23 +113,21 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
   }
   const bool two = c1 < p.D;  // the last copied chunk may hold one vector
   for (int i = threadIdx.x; i < kChunks * V; i += kThreads) {
-    const int64_t n = first + i / V, r = n / p.chunks;
-    const int k = (int)(n % p.chunks);
-    if (r < rows && k < p.rot_chunks) {
-      double turn = (double)p.pos[r / p.T * p.ps_b + r % p.T * p.ps_t] * (double)p.inv_freq[V * k + i % V] *
-                    0.15915494309189533577;  // 1 / (2 pi)
-      turn -= rint(turn);
+    const int k = chunk[i / V];
+    if (k < p.rot_chunks) {
+      double turn = where[i / V] * (double)p.inv_freq[V * k + i % V];
+      turn -= (turn + 6755399441055744.0) - 6755399441055744.0;  // 1.5 * 2^52: rounds to whole turns
       float s, co;
       sincospif((float)(2.0 * turn), &s, &co);
       turns[i] = make_float2(co * p.scale, s * p.scale * p.sgn);
     }
   }
   __syncthreads();
-  if (!live) return;
+  if (b < 0) return;
   float cs[V], sn[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const float2 f = turns[threadIdx.x % kChunks * V + i];
+    const float2 f = turns[mine * V + i];
     cs[i] = f.x;
     sn[i] = f.y;
   }
@@ -175,7 +183,7 @@ int launch(RotaryParams& p, bool inter, cudaStream_t stream) {
   p.rot_chunks = p.r / (2 * V);
   p.chunks = p.rot_chunks + ceil_div(p.D - p.r, 2 * V);
   const int64_t blocks = ceil_div64((int64_t)p.B * p.T * p.chunks, kChunks);
-  if (blocks > 0x7fffffff) return SKV_ERR_UNSUPPORTED;
+  if (blocks > 0x7fffffff || (int64_t)p.B * p.T > 0x7fffffff) return SKV_ERR_UNSUPPORTED;
   // a small call wants its heads side by side
   p.heads_per_block = align_up(p.H, kHeads);
   while (p.heads_per_block > kHeads && blocks * ceil_div(p.H, p.heads_per_block) < 8 * 148)
