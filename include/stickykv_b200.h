@@ -285,7 +285,7 @@ int skv_pack_pages(const skv_layer_desc* layer, const void* k, const void* v, in
  * inverse != 0 takes -a (same scale).  Channels r.. are copied.  Arithmetic in
  * fp32, one rounding to dtype.  Each output may be its own input (same
  * pointer and strides: in place); otherwise outputs and inputs must not
- * overlap.  k == NULL: queries only.
+ * overlap.  k == NULL: queries only.  batch * tokens is below 2^31.
  */
 typedef struct skv_rotary_args {
   int32_t batch, tokens, num_q_heads, num_kv_heads, head_dim, rotary_dim;
@@ -312,12 +312,14 @@ int skv_rotary(const skv_rotary_args* args, void* stream);
  * slot p = query_slots[b] + i (NULL: ends[b] - q_tokens + i).  It sees key j
  * when
  *   starts <= j <= p < ends and (j - starts < sinks or p - j < window),
- * out = softmax(scaling * q·k) v over the keys it sees, 0 when it sees none.
+ * out = softmax(scaling * q·k) v over the keys it sees, 0 when it sees none
+ * or every score is -inf.
  * Keys and values that a query does not see never reach its output, whatever
  * they hold.  q/k/v: [batch][heads][tokens or slots][head_dim] in dtype, unit
  * stride along head_dim, 16-byte aligned base and strides; out
  * [batch][q_tokens][num_q_heads][head_dim] contiguous.  head_dim 16, 32, 64
- * or 128.
+ * or 128; batch and heads up to 65535, q_tokens and k_slots up to 2^29, and
+ * q_tokens times the query heads of a kv head below 2^31.
  */
 typedef struct skv_window_args {
   int32_t batch, q_tokens, k_slots, num_q_heads, num_kv_heads, head_dim, dtype;

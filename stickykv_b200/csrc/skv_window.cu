@@ -45,6 +45,8 @@ int check_window(const skv_window_args* a) {
   // heads and rows index grid dimensions; slots and queries 31-bit sums
   if (a->batch > 65535 || a->num_q_heads > 65535 || a->k_slots > (1 << 29) || a->q_tokens > (1 << 29))
     return SKV_ERR_UNSUPPORTED;
+  // so do the (token, head) pairs of a kv head
+  if ((int64_t)a->q_tokens * (a->num_q_heads / a->num_kv_heads) > 0x7fffffff) return SKV_ERR_UNSUPPORTED;
   const void* ptrs[4] = {a->q, a->k, a->v, a->out};
   for (const void* x : ptrs)
     if ((uintptr_t)x % 16) return SKV_ERR_MISALIGNED;

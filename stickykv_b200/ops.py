@@ -302,8 +302,9 @@ def sink_window_attention(query: Tensor, key: Tensor, value: Tensor, *, window: 
     starts < sinks`` or ``p - j < window`` (``window=None``: every earlier
     token).  So a left-padded prompt gives ``starts``, a right-padded one
     ``ends`` and zero ``query_slots``, a decode step over a preallocated cache
-    ``ends``.  A query that sees no key (padding) gets zeros; what a query does
-    not see never reaches its output, whatever it holds."""
+    ``ends``.  A query that sees no key (padding), or only scores of -inf,
+    gets zeros; what a query does not see never reaches its output, whatever
+    it holds."""
     plan_key = None
     if out is None:
         index = query.get_device()
@@ -417,7 +418,7 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
                 check(lib().skv_sample(C.byref(a), _raw_stream(index)), "skv_sample")
                 return out
     _same_device("sample_tokens", logits.device, uniform=uniform, out=out)
-    _no_grad("sample_tokens", logits, uniform)
+    _no_grad("sample_tokens", logits, uniform, *(s for s in (temperature, top_k, top_p, min_p) if torch.is_tensor(s)))
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"sample_tokens: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
     dt = _DT.get(logits.dtype)

@@ -280,6 +280,34 @@ def test_window_unseen_tokens_may_hold_anything(dt, D, T, rows):
     within(got[:, ~hit], ref[0][:, ~hit], window_tol(q, ref)[:, ~hit])
 
 
+@pytest.mark.parametrize("dt, D, T", [("f32", 32, 200), ("f16", 16, 9), ("f16", 64, 200), ("bf16", 128, 333), ("f16", 128, 1), ("bf16", 64, 3)])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_window_scores_of_minus_infinity(dt, D, T, rows):
+    """A key whose score is -inf weighs nothing; a query of such keys alone
+    gives zeros.  Without its infinite channel a key's score is -10^4 / sqrt(D)
+    or below -800 and its 64-bit weight beside another key's exactly 0."""
+    S, window = 333, 40
+    q, k, v = qkv(rows, T, S, 4, 2, D, dt, 5)
+    q[..., 0] = 1
+    gone = torch.zeros(S, dtype=torch.bool, device="cuda")
+    gone[::3] = True
+    gone[S - 41:] = True
+    gone[S - 150:S - 100] = True
+    clean, low = k.clone(), k.clone()
+    k[:, :, gone, 0] = -math.inf
+    low[:, :, gone, 0] = -1e4
+    clean[:, :, gone, 0] = 0
+    p = torch.arange(S - T, S, device="cuda")[:, None]
+    j = torch.arange(S, device="cuda")
+    for sinks in (0, 2):
+        got = skv.sink_window_attention(q, k, v, window=window, sinks=sinks)
+        some = ((j <= p) & ((p - j < window) | (j < sinks)) & ~gone).any(1)
+        assert (sinks == 2 or not some.all()) and not got[:, ~some].any()
+        out, A, _, n = window_ref(q, low, v, window, sinks)
+        d = window_ref(q, clean, v, window, sinks)[2]
+        within(got[:, some], out[:, some], window_tol(q, (out, A, d, n))[:, some])
+
+
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("B, T", [(2, 1), (2, 40), (60, 150)])
 def test_window_strides(dt, B, T):

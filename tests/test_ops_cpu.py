@@ -124,6 +124,12 @@ def test_sample_refusals(kw, error):
         _sample(**kw)
 
 
+@pytest.mark.parametrize("name", ["temperature", "top_p", "min_p"])
+def test_sample_refuses_gradients_of_settings(name):
+    with pytest.raises(NotImplementedError, match="no backward"):
+        _sample(**{name: torch.full((2,), 0.5, requires_grad=True)})
+
+
 # -- C entries: every refusal comes before anything is launched ---------------------------
 
 _P = 1 << 20  # an aligned address that nothing reads
@@ -169,6 +175,13 @@ def test_window_c_refusals(kw, status):
     L = _lib.lib()
     assert L.skv_window_attention(C.byref(_window_args(**kw)), None) == status
     assert L.skv_window_attention(None, None) == 1
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q_tokens=(1 << 29) + 1), dict(k_slots=(1 << 29) + 1), dict(q_tokens=1 << 29, num_q_heads=8),
+])
+def test_window_c_refuses_what_31_bits_do_not_hold(kw):
+    assert _lib.lib().skv_window_attention(C.byref(_window_args(**kw)), None) == 2
 
 
 @pytest.mark.parametrize("kw, status", [
