@@ -42,6 +42,7 @@ constexpr int kPerThread = kBins / kThreads;
 constexpr int kList = 2048;        // tokens that are searched in registers, 4 a thread
 constexpr int kRanked = 192;       // listed tokens up to here are compared each with each (n^2 / 512 steps a thread; more take
                                    // three to four turns of 8 bits, about 1.5 us each)
+constexpr int kLists = 4;          // made for a row at most: two for top-k, two for top-p
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kNone = 0x007fffffu;  // key of -inf
 constexpr double kUnit = 4503599627370496.0;  // 2^52: a listed weight as a whole number
@@ -148,8 +149,8 @@ struct Shared {
   uint64_t warp_best[kWarps];             // of each warp: largest key above the complement of its first block's place
   uint32_t warp_least[kWarps];            // smallest key
   uint32_t warp_min[kWarps];              // smallest of its lanes' largest keys
-  uint32_t listed[3];
-  uint32_t list_lo[3], list_hi[3];        // smallest and largest listed key
+  uint32_t listed[kLists];
+  uint32_t list_lo[kLists], list_hi[kLists];        // smallest and largest listed key
   uint32_t finite;                        // smallest key above -inf, where the row holds such
   uint32_t list_above;                    // tokens above the list
   double mass[2];                         // above the bracket; below its upper end
@@ -387,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       sh.warp_least[warp] = low;
       sh.warp_min[warp] = lane_min;
     }
-    if (tid < 3) {
+    if (tid < kLists) {
       sh.listed[tid] = 0;
       sh.list_lo[tid] = 0xffffffffu;
       sh.list_hi[tid] = 0;
@@ -876,54 +877,75 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
       }
       float reached = block_prefix(s) - s;
       const float all = block_reduce(reached + s, Max()) + (tau ? (float)ties * (float)safe_weight(tau) * 16384.f : 0.f);
+      int short_of = -1;  // the last bin that does not reach the cut
 #pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        if (reached < share * all && (reached += mass[i]) >= share * all) atomicMax(&sh.last, tid * kPerThread + i);
-      }
+      for (int i = 0; i < kPerThread; ++i)
+        if ((reached += mass[i]) < share * all) short_of = tid * kPerThread + i;
+      short_of = __reduce_max_sync(0xffffffffu, short_of);
+      if (lane == 0 && short_of >= 0) atomicMax(&sh.last, short_of);
       __syncthreads();
-      // the bracket: that bin and a little beyond.  Exactly: the mass above it and that of all kept tokens
-      const int bin = max(sh.last, 0);
-      const float unit = per_unit > 0.f ? 1.f / per_unit : 0.f;
-      const float low = m - ((float)bin + 0.65f) * unit, high = m - ((float)bin - 0.65f) * unit;
-      double above = 0, rest = 0, above2 = 0, rest2 = 0;
-      const uint32_t n = collect(
-          kept_from, low, high,
-          [&](const float (&v)[8]) {
-            double e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = weight(v[i]);
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-              if (v[i] > high) above += e[i];
-              if (v[i + 1] > high) above2 += e[i + 1];
-              if (v[i] <= high && v[i] >= kept_from) rest += e[i];
-              if (v[i + 1] <= high && v[i + 1] >= kept_from) rest2 += e[i + 1];
-            }
-          },
-          [&] {
-            above = block_reduce(above + above2, Sum());
-            rest = block_reduce(rest + rest2, Sum());
-            if (tid == 0) {
-              sh.mass[0] = above;
-              sh.mass[1] = rest;
-            }
-          });
-      above = over(&sh.mass[0], Sum());
-      rest = over(&sh.mass[1], Sum());
+      int bin = min(sh.last + 1, kBins - 1);
       const float v_tau = tau ? value_of(tau) : -INFINITY;
-      const double goal = (double)share * (above + rest + (tau ? ties * safe_weight(tau) : 0.0)) - above;
-      const bool ends_here = tau && v_tau >= low && v_tau <= high;
+      if (tau) bin = min(bin, (int)bin_at(place(depth(v_tau))));  // nothing is kept below
+      const float unit = per_unit > 0.f ? 1.f / per_unit : 0.f;
       bool found = false;
-      if (goal > 0 && goal < 1024.0 && n > 0 && n <= kList && v_tau <= high) {  // 2^10 * 2^52 and the list's 2^63 fit 64 bits
-        listed_weights();
-        found = cut(ends_here ? ties * w_tau : 0, (uint64_t)max(1ll, __double2ll_ru(goal * kUnit)));
-      } else if (goal > 0 && n > kList && list_lo == list_hi && list_lo > tau && list_lo >= low_key) {  // equals only
-        const double need = ceil(goal / weight(value_of(list_lo)));
-        if (need <= (double)n) {
-          tau = list_lo;
-          ties = (uint32_t)need;
-          found = true;
+      // The histogram's sums are off by 10^-7 of the whole and more: a cut at the very end of a bin, as one of some
+      // thousand 16-bit rows has it, may be in the next one that holds tokens, which the exact sums tell (one such row
+      // among 128, searched bit by bit instead, made 434 us of 120)
+#pragma unroll 1
+      for (int attempt = 0; bin >= 0 && bin < kBins; ++attempt) {
+        // the bracket: that bin and a little beyond.  Exactly: the mass above it and that of all kept tokens
+        const float low = m - ((float)bin + 0.65f) * unit, high = m - ((float)bin - 0.65f) * unit;
+        double above = 0, rest = 0, above2 = 0, rest2 = 0;
+        const uint32_t n = collect(
+            kept_from, low, high,
+            [&](const float (&v)[8]) {
+              double e[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) e[i] = weight(v[i]);
+#pragma unroll
+              for (int i = 0; i < 8; i += 2) {
+                if (v[i] > high) above += e[i];
+                if (v[i + 1] > high) above2 += e[i + 1];
+                if (v[i] <= high && v[i] >= kept_from) rest += e[i];
+                if (v[i + 1] <= high && v[i + 1] >= kept_from) rest2 += e[i + 1];
+              }
+            },
+            [&] {
+              above = block_reduce(above + above2, Sum());
+              rest = block_reduce(rest + rest2, Sum());
+              if (tid == 0) {
+                sh.mass[0] = above;
+                sh.mass[1] = rest;
+              }
+            });
+        above = over(&sh.mass[0], Sum());
+        rest = over(&sh.mass[1], Sum());
+        const double goal = (double)share * (above + rest + (tau ? ties * safe_weight(tau) : 0.0)) - above;
+        const bool ends_here = tau && v_tau >= low && v_tau <= high;
+        if (goal > 0 && goal < 1024.0 && n > 0 && n <= kList && v_tau <= high) {  // 2^10 * 2^52 and the list's 2^63 fit 64 bits
+          listed_weights();
+          found = cut(ends_here ? ties * w_tau : 0, (uint64_t)max(1ll, __double2ll_ru(goal * kUnit)));
+        } else if (goal > 0 && n > kList && list_lo == list_hi && list_lo > tau && list_lo >= low_key) {  // equals only
+          const double need = ceil(goal / weight(value_of(list_lo)));
+          if (need <= (double)n) {
+            tau = list_lo;
+            ties = (uint32_t)need;
+            found = true;
+          }
         }
+        if (found || attempt > 0 || (goal > 0 && n > kList)) break;
+        cluster_barrier();  // what the others read of this block is written anew
+        if (tid == 0) sh.last = goal > 0 ? kBins : -1;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+          const int at = tid * kPerThread + i;
+          if (mass[i] > 0.f && goal > 0 && at > bin) atomicMin(&sh.last, at);
+          if (mass[i] > 0.f && !(goal > 0) && at < bin) atomicMax(&sh.last, at);
+        }
+        __syncthreads();
+        bin = sh.last;
       }
       if (!found) slow_mass(share);
     }

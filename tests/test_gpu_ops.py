@@ -521,6 +521,26 @@ def test_sample_cuts_among_equals(dt):
         check_sample(x, u, **kw)
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("step, levels, many", [(0.5, 16, 13), (0.25, 30, 200), (2.0, 6, 3), (0.015625, 64, 20)])
+def test_sample_cuts_between_levels(step, levels, many, dt):
+    """Shares of top-p one step of float32 to each side of a level's end, and
+    nearest to it: 32-bit sums cannot tell which level holds the cut.  The
+    vocabulary ascends, so that a random number of 0 draws the cut's level."""
+    counts = [1 + many * j for j in range(levels)]
+    x = torch.cat([torch.full((n,), 4.0 - step * j) for j, n in reversed(list(enumerate(counts)))])
+    mass = np.cumsum([n * np.exp(-step * j) for j, n in enumerate(counts)])
+    ends = (mass[:-1] / mass[-1]).astype(np.float32)
+    shares = np.concatenate([np.nextafter(ends, np.float32(0)), ends, np.nextafter(ends, np.float32(1))])
+    assert np.abs(shares.astype(np.float64)[:, None] - mass[:-1] / mass[-1]).min() > 1e-13  # 64-bit sums can tell
+    B = len(shares)
+    x = x.to(DT[dt]).cuda().expand(B, -1)
+    top_p = torch.from_numpy(shares).cuda()
+    for u in (torch.zeros(B, device="cuda"), torch.rand(B, generator=gen(levels), device="cuda")):
+        check_sample(x, u, top_p=top_p)
+        check_sample(x, u, top_p=top_p, top_k=x.shape[1] - 1)
+
+
 def test_sample_extreme_scales():
     """Logits and temperatures near the ends of their types."""
     g = gen(41)
