@@ -941,8 +941,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
 #pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
           const int at = tid * kPerThread + i;
-          if (mass[i] > 0.f && goal > 0 && at > bin) atomicMin(&sh.last, at);
-          if (mass[i] > 0.f && !(goal > 0) && at < bin) atomicMax(&sh.last, at);
+          if (!(gathered[0][at] + gathered[1][at] > 0.f)) continue;
+          if (goal > 0 && at > bin) atomicMin(&sh.last, at);
+          if (!(goal > 0) && at < bin) atomicMax(&sh.last, at);
         }
         __syncthreads();
         bin = sh.last;
