@@ -51,6 +51,9 @@ __device__ __forceinline__ void window_join(const WindowParams& p, const WindowR
         sum += f * stat[(kWarps + 1 + w) * kRows + r];
         val += f * part[(size_t)w * kRows * kPitch + r * kPitch + d];
       }
+    } else {  // no score above -inf: the sums are 0, but NaN where a score was (a maximum passes over those)
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) sum += stat[(kWarps + 1 + w) * kRows + r];
     }
     part[r * kPitch + d] = val;
     if (d == 0) {
@@ -77,7 +80,10 @@ __device__ __forceinline__ void window_join(const WindowParams& p, const WindowR
         const float mz = ld_cluster(s_stat + (kWarps * kRows + r) * 4, z);
         const float lz = ld_cluster(s_stat + ((2 * kWarps + 1) * kRows + r) * 4, z);
         const float vz = ld_cluster(s_part + (r * kPitch + d) * 4, z);
-        if (mz == -INFINITY) continue;
+        if (mz == -INFINITY) {
+          sum += lz;  // 0 or NaN, as above
+          continue;
+        }
         const float mn = fmaxf(mx, mz), f0 = ex2(mx - mn), f1 = ex2(mz - mn);
         sum = sum * f0 + lz * f1;
         val = val * f0 + vz * f1;

@@ -308,6 +308,59 @@ def test_window_scores_of_minus_infinity(dt, D, T, rows):
         within(got[:, some], out[:, some], window_tol(q, (out, A, d, n))[:, some])
 
 
+@pytest.mark.parametrize("dt, D", [("f32", 16), ("f32", 64), ("f32", 128), ("f16", 16), ("f16", 64), ("bf16", 32), ("bf16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("T, rows, window", [(1, 1, 40), (1, 40, 40), (3, 1, 40), (200, 1, 40), (200, 40, 40), (333, 60, 170)])
+def test_window_scores_that_are_not_finite(dt, D, T, rows, window):
+    """A NaN among the scores a query sees, or one of +inf, makes its output
+    NaN, as the softmax of such scores is, whatever its other scores are; the
+    outputs of the other queries stay."""
+    S = 333
+    q, k, v = qkv(rows, T, S, 4, 2, D, dt, 11)
+    ref = window_ref(q, k, v, window, 2)
+    tol = window_tol(q, ref)
+    one = q.clone()
+    one[:, 1, T - 1, 3] = math.nan                 # every score of one query
+    got = skv.sink_window_attention(one, k, v, window=window, sinks=2)
+    hit = torch.zeros(rows, T, 4, dtype=torch.bool, device="cuda")
+    hit[:, T - 1, 1] = True
+    assert got[hit].isnan().all()
+    within(got[~hit], ref[0][~hit], tol[~hit])
+    # a key that is all a query sees
+    bad = k.clone()
+    bad[:, 0, S - 1, 0] = math.nan
+    alone = window_ref(q, k, v, 1, 0)
+    got = skv.sink_window_attention(q, bad, v, window=1)
+    hit = torch.zeros(rows, T, 4, dtype=torch.bool, device="cuda")
+    hit[:, T - 1, :2] = True                       # the heads that share kv head 0
+    assert got[hit].isnan().all()
+    within(got[~hit], alone[0][~hit], window_tol(q, alone)[~hit])
+    # scores of +inf and of NaN that some queries see
+    q[..., 0] = 1
+    ref = window_ref(q, k, v, window, 2)
+    tol = window_tol(q, ref)
+    p = torch.arange(S - T, S, device="cuda")
+    for value in (math.inf, math.nan):
+        for j in (S - 1, S - 60, 1):
+            bad = k.clone()
+            bad[:, :, j, 0] = value
+            got = skv.sink_window_attention(q, bad, v, window=window, sinks=2)
+            hit = (j <= p) & ((p - j < window) | (j < 2))
+            assert got[:, hit].isnan().all(), (value, j)
+            within(got[:, ~hit], ref[0][:, ~hit], tol[:, ~hit], f"{value} at {j}")
+
+
+@pytest.mark.parametrize("dt, D", [("f32", 16), ("f32", 128), ("f16", 32), ("bf16", 64), ("f16", 128)])
+@pytest.mark.parametrize("lo, hi", [(0, 300), (0, 1), (3999, 4000), (1000, 4000), (0, 4000), (2000, 2256)])
+def test_window_whole_shares_of_scores_that_are_nan(dt, D, lo, hi):
+    """Decode of a row whose keys are shared out over many warps and blocks,
+    some of which see NaN and nothing else."""
+    q, k, v = qkv(1, 1, 4000, 4, 2, D, dt, 12)
+    want = skv.sink_window_attention(q, k, v)
+    k[:, 1, lo:hi] = math.nan
+    got = skv.sink_window_attention(q, k, v)
+    assert got[:, :, 2:].isnan().all() and torch.equal(got[:, :, :2], want[:, :, :2])
+
+
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("B, T", [(2, 1), (2, 40), (60, 150)])
 def test_window_strides(dt, B, T):
