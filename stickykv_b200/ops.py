@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 from typing import Any, Dict, Optional, Tuple, Union
 
 import torch
@@ -67,6 +68,16 @@ def _cuda(what: str, device: torch.device) -> None:
 def _no_grad(what: str, *tensors: Optional[Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError(f"{what} has no backward pass: call it under torch.no_grad()")
+
+
+def _setting(what: str, x: Any, kind: type) -> Any:
+    """A setting as the plain number it is now (None stays): a 0-dim tensor would
+    be found again by its identity, whatever it holds by then."""
+    if x is None or x.__class__ is kind:
+        return x
+    if torch.is_tensor(x):
+        _no_grad(what, x)
+    return int(operator.index(x)) if kind is int else kind(x)
 
 
 def _overlap(a: Tensor, b: Tensor) -> bool:
@@ -171,6 +182,9 @@ def apply_rotary(query: Tensor, key: Optional[Tensor], positions: Tensor, inv_fr
     rotated channels; ``inverse`` turns back (and still multiplies by
     ``scale``).  ``out`` gives the outputs' tensors; each may be its own input
     (in place) and must otherwise not overlap any input."""
+    if not (interleaved.__class__ is inverse.__class__ is bool and scale.__class__ is float):
+        interleaved, inverse = _setting("apply_rotary", interleaved, bool), _setting("apply_rotary", inverse, bool)
+        scale = _setting("apply_rotary", scale, float)
     plan_key = None
     if out is None:
         index = query.get_device()
@@ -305,6 +319,9 @@ def sink_window_attention(query: Tensor, key: Tensor, value: Tensor, *, window: 
     ``ends``.  A query that sees no key (padding), or only scores of -inf,
     gets zeros; what a query does not see never reaches its output, whatever
     it holds."""
+    if window.__class__ is not int or sinks.__class__ is not int or scaling is not None:
+        window, sinks = _setting("sink_window_attention", window, int), _setting("sink_window_attention", sinks, int)
+        scaling = _setting("sink_window_attention", scaling, float)
     plan_key = None
     if out is None:
         index = query.get_device()
@@ -399,14 +416,18 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
     or below 0 or NaN is greedy, a top_k at or below 0, a top_p from 1 on and
     a min_p at or below 0 cut nothing, a top_p at or below 0 keeps one token.
     The largest token is always kept.  V is at most 4,194,304."""
+    # `tensors` holds each setting that is one for every row, None for a number; it is empty where all are numbers
+    settings, tensors = (temperature, top_k, top_p, min_p), ()
+    if not (top_k.__class__ is int and temperature.__class__ is top_p.__class__ is min_p.__class__ is float):
+        tensors = tuple(s if torch.is_tensor(s) else None for s in settings)
+        settings = tuple(s if t is not None else _setting("sample_tokens", s, kind)
+                         for s, t, kind in zip(settings, tensors, (float, int, float, float)))
     plan_key = None
     if out is None:
         index = logits.get_device()
-        tensors = [None if s.__class__ in (int, float) else s if torch.is_tensor(s) else None
-                   for s in (temperature, top_k, top_p, min_p)]
         if _ready(index, logits, uniform, *tensors):
-            plan_key = ("sample", logits.dtype, logits.shape, logits.stride(), _meta(uniform)) + tuple(
-                s if t is None else _meta(t) for s, t in zip((temperature, top_k, top_p, min_p), tensors))
+            plan_key = ("sample", logits.dtype, logits.shape, logits.stride(), _meta(uniform),
+                        settings if not tensors else tuple(s if t is None else _meta(t) for s, t in zip(settings, tensors)))
             plan = _PLANS.get(plan_key)
             if plan is not None:
                 a = SampleArgs.from_buffer_copy(plan)
@@ -418,7 +439,7 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
                 check(lib().skv_sample(C.byref(a), _raw_stream(index)), "skv_sample")
                 return out
     _same_device("sample_tokens", logits.device, uniform=uniform, out=out)
-    _no_grad("sample_tokens", logits, uniform, *(s for s in (temperature, top_k, top_p, min_p) if torch.is_tensor(s)))
+    _no_grad("sample_tokens", logits, uniform, *tensors)
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"sample_tokens: logits must be [rows, vocabulary], got {tuple(logits.shape)}")
     dt = _DT.get(logits.dtype)
@@ -430,8 +451,8 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
     if out is not None and (out.dtype != torch.int64 or out.shape != (B,) or not out.is_contiguous()):
         raise ValueError(f"sample_tokens: out must be a contiguous int64 tensor of shape [{B}]")
     values, arrays = [], []
-    for name, s, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+    for name, s, dtype in zip(("temperature", "top_k", "top_p", "min_p"), settings,
+                              (torch.float32, torch.int32, torch.float32, torch.float32)):
         if torch.is_tensor(s):
             if s.device != logits.device or s.dtype != dtype or s.shape != (B,) or not s.is_contiguous():
                 raise ValueError(f"sample_tokens: {name} must be a number or a contiguous {dtype} tensor of shape "

@@ -437,6 +437,32 @@ def test_window_repeated_calls_are_checked_again():
         skv.sample_tokens(x, u.cpu(), top_k=5)
 
 
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+def test_settings_in_tensors_are_read_at_each_call(device):
+    """A setting given as a 0-dim tensor counts with what it holds at the call."""
+    q, k, v = qkv(2, 1, 64, 4, 2, 64, "f16", 1)
+    inv, _ = skv.rotary_frequencies(64, device="cuda")
+    pos = torch.arange(5, 6, device="cuda")
+    x, u = normal((2, 99), torch.float32, gen(2)), torch.rand(2, generator=gen(3), device="cuda")
+    attend = lambda **kw: skv.sink_window_attention(q, k, v, **kw)  # noqa: E731
+    rotate = lambda **kw: skv.apply_rotary(q, None, pos, inv, **kw)[0]  # noqa: E731
+    for call, name, values in ((attend, "scaling", (0.125, 0.5)), (attend, "window", (9, 30)), (rotate, "scale", (1.0, 0.75)),
+                               (rotate, "inverse", (False, True)), (rotate, "interleaved", (False, True))):
+        other = {"window": 20} if call is attend and name != "window" else {}
+        want = [call(**{name: y}, **other) for y in values]
+        assert not torch.equal(*want)
+        t = torch.tensor(values[0], device=device)
+        for y, w in ((values[0], want[0]), (values[1], want[1]), (values[0], want[0])):
+            t.fill_(y)
+            for _ in range(2):
+                assert torch.equal(call(**{name: t}, **other), w), (name, y)
+    few = torch.tensor(3, device=device)
+    want = [attend(window=5, sinks=n) for n in (3, 11)]
+    assert torch.equal(attend(window=5, sinks=few), want[0]) and torch.equal(attend(window=5, sinks=few.fill_(11)), want[1])
+    top_k = np.int64(4)
+    assert torch.equal(skv.sample_tokens(x, u, top_k=top_k), skv.sample_tokens(x, u, top_k=4))
+
+
 def test_window_past_32_bit_offsets():
     """A cache of over 2^31 elements, most of it never written; decode and a
     chunk at its far end and, with sinks, at its beginning."""

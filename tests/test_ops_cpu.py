@@ -130,6 +130,18 @@ def test_sample_refuses_gradients_of_settings(name):
         _sample(**{name: torch.full((2,), 0.5, requires_grad=True)})
 
 
+@pytest.mark.parametrize("call, kw, error", [
+    (_rotary, dict(inverse=torch.ones(2)), RuntimeError), (_window, dict(window=4.0), TypeError), (_window, dict(sinks=1.5), TypeError),
+    (_window, dict(window=torch.tensor(4.0)), TypeError), (_window, dict(scaling="x"), ValueError),
+    (_window, dict(scaling=torch.tensor(0.5, requires_grad=True)), NotImplementedError),
+    (_sample, dict(top_k=2.0), TypeError), (_sample, dict(temperature="x"), ValueError),
+    (_sample, dict(top_p=torch.tensor(0.5)), ValueError),
+])
+def test_settings_are_numbers(call, kw, error):
+    with pytest.raises(error):
+        call(**kw)
+
+
 # -- C entries: every refusal comes before anything is launched ---------------------------
 
 _P = 1 << 20  # an aligned address that nothing reads
