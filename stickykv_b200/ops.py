@@ -95,14 +95,25 @@ def _overlap(a: Tensor, b: Tensor) -> bool:
 
 # -- rotary positions ------------------------------------------------------------------
 
-def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optional[Dict[str, Any]] = None,
+# what a dict of rotary settings may hold; a key from elsewhere could ask for other frequencies
+_ROPE_KEYS = frozenset((
+    "rope_type", "type", "rope_theta", "partial_rotary_factor", "factor", "original_max_position_embeddings",
+    "low_freq_factor", "high_freq_factor", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale",
+    "mscale_all_dim"))
+
+
+def rotary_frequencies(rotary_dim: int, theta: Optional[float] = None, scaling: Optional[Dict[str, Any]] = None,
                        seq_len: Optional[int] = None, device: Union[str, torch.device, None] = None
                        ) -> Tuple[Tensor, float]:
     """``(inv_freq, scale)`` of :func:`apply_rotary`: the angle per position of
     each of the ``rotary_dim / 2`` pairs (float32, computed in 64 bits) and the
     factor on cosine and sine.
 
-    ``scaling`` takes transformers' ``rope_scaling`` dicts by ``rope_type``:
+    ``scaling`` takes transformers' ``rope_scaling`` dicts.  ``theta`` is the
+    dict's ``rope_theta`` where that is given, else 10000; two that differ are
+    refused, and so is a key that is not known here, or a
+    ``partial_rotary_factor`` other than 1 (the part of a head that is rotated
+    is ``rotary_dim``).  By ``rope_type``:
 
     * ``"default"`` (or None): ``f_i = theta^(-2i/r)``;
     * ``"linear"``: ``f_i / factor``;
@@ -113,14 +124,26 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
       ``original / high_freq_factor`` kept, those between blended;
     * ``"yarn"``: blended over the pair index between ``beta_fast`` and
       ``beta_slow`` turns in the original context; ``scale`` is
-      ``attention_factor``, by default ``0.1 ln(factor) + 1``."""
+      ``attention_factor``, by default ``g(1)`` of ``g(m) = 0.1 m ln(factor) +
+      1``, or ``g(mscale) / g(mscale_all_dim)`` where both are given and not 0."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be a positive even number, got {rotary_dim}")
+    cfg = {name: v for name, v in (scaling or {}).items() if v is not None}
+    kind = cfg.get("rope_type", cfg.get("type", "default"))
+    unknown = sorted(str(name) for name in cfg if name not in _ROPE_KEYS)
+    if unknown:
+        raise NotImplementedError(f"rope_type {kind!r} with {', '.join(unknown)} is not supported")
+    given = cfg.get("rope_theta")
+    if theta is None:
+        theta = 10000.0 if given is None else given
+    elif given is not None and given != theta:
+        raise ValueError(f"theta is {theta}, the dict's rope_theta {given}")
     if not theta > 0 or not math.isfinite(theta):
         raise ValueError(f"theta must be positive and finite, got {theta}")
+    if cfg.get("partial_rotary_factor", 1.0) != 1.0:
+        raise ValueError(f"partial_rotary_factor {cfg['partial_rotary_factor']}: give the rotated channels as rotary_dim "
+                         "and leave it out")
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
-    cfg = dict(scaling or {})
-    kind = cfg.get("rope_type", cfg.get("type", "default"))
 
     def need(name: str) -> float:
         v = cfg.get(name)
@@ -162,8 +185,15 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
         lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
         ramp = ((i / 2 - lo) / (hi - lo if hi != lo else 0.001)).clamp(0.0, 1.0)
         freq = freq * ((1.0 - ramp) + ramp / factor)
-        given = cfg.get("attention_factor")
-        scale = float(given) if given is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+        def growth(m: float) -> float:
+            return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+        if "attention_factor" in cfg:
+            scale = float(cfg["attention_factor"])
+        elif cfg.get("mscale") and cfg.get("mscale_all_dim"):
+            scale = growth(need("mscale")) / growth(need("mscale_all_dim"))
+        else:
+            scale = growth(1.0)
     elif kind != "default":
         raise NotImplementedError(f"rope_type {kind!r} is not supported")
     return freq.to(torch.float32).to(device if device is not None else "cpu"), scale

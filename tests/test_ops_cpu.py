@@ -266,3 +266,52 @@ def test_frequency_refusals(kw, error):
     a.update(kw)
     with pytest.raises(error):
         skv.rotary_frequencies(**a)
+
+
+_YARN = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
+
+
+@pytest.mark.parametrize("scaling", [
+    dict(_YARN, mscale=1.0, mscale_all_dim=1.0), dict(_YARN, mscale=0.707, mscale_all_dim=1.0),
+    dict(_YARN, mscale=1.0, mscale_all_dim=0.707), dict(_YARN, mscale=0.707), dict(_YARN, mscale_all_dim=0.707),
+    dict(_YARN, mscale=0.0, mscale_all_dim=1.0), dict(_YARN, mscale=1.0, mscale_all_dim=0.707, attention_factor=1.1),
+    dict(_YARN, factor=1.0, mscale=0.5, mscale_all_dim=1.0), dict(_YARN, attention_factor=None, mscale=2.0, mscale_all_dim=0.5),
+    dict(_YARN, beta_fast=16.0, truncate=False), {"rope_type": "default"},
+    {"rope_type": "linear", "factor": 4.0, "original_max_position_embeddings": 512},
+])
+def test_frequencies_of_whole_dicts_are_those_of_transformers(scaling):
+    """Dicts as a configuration holds them, theta among them; bounds as above."""
+    from transformers import LlamaConfig
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+    dim = 64
+    original = scaling.get("original_max_position_embeddings", 512)
+    params = dict(scaling, rope_theta=500000.0)
+    cfg = LlamaConfig(hidden_size=2 * dim, num_attention_heads=2, head_dim=dim, max_position_embeddings=original,
+                      rope_parameters=params)
+    if scaling["rope_type"] == "default":
+        want, want_scale = 1.0 / 500000.0 ** (torch.arange(0, dim, 2).double() / dim), 1.0
+    else:
+        want, want_scale = ROPE_INIT_FUNCTIONS[scaling["rope_type"]](cfg, torch.device("cpu"))
+    for inv, scale in (skv.rotary_frequencies(dim, scaling=params), skv.rotary_frequencies(dim, 500000.0, params),
+                       skv.rotary_frequencies(dim, 500000.0, scaling), skv.rotary_frequencies(dim, scaling=cfg.rope_parameters)):
+        assert torch.allclose(inv.double(), want.double(), rtol=32 * 2.0 ** -24, atol=0)
+        assert scale == pytest.approx(want_scale, rel=1e-6)
+
+
+def test_default_theta():
+    for args in ((), (None,), (10000,), (None, {}), (None, {"rope_theta": None})):
+        assert torch.equal(skv.rotary_frequencies(64, *args)[0], skv.rotary_frequencies(64, 10000.0)[0])
+
+
+@pytest.mark.parametrize("theta, scaling, error", [
+    (10000.0, {"rope_type": "default", "rope_theta": 500000.0}, ValueError),
+    (None, {"rope_theta": -1.0}, ValueError),
+    (None, {"rope_type": "default", "partial_rotary_factor": 0.5}, ValueError),
+    (None, {"rope_type": "dynamic", "factor": 1.0, "original_max_position_embeddings": 512, "alpha": 1000.0}, NotImplementedError),
+    (None, dict(_YARN, some_factor=2.0), NotImplementedError),
+    (None, dict(_YARN, mscale=-1.0, mscale_all_dim=1.0), ValueError),
+    (None, dict(_YARN, mscale=1.0, mscale_all_dim=math.nan), ValueError),
+])
+def test_frequency_dicts_that_are_refused(theta, scaling, error):
+    with pytest.raises(error):
+        skv.rotary_frequencies(64, theta, scaling)
