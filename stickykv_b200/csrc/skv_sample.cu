@@ -959,8 +959,28 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   if (min_p > 0.f && min_p < 1.f) {
     from_key = key_of((float)((double)m + log((double)min_p) * (double)temp));
     from_key = min(max(from_key, low_key), top);
-    while (from_key > low_key && weight(value_of(from_key - 1)) >= (double)min_p) --from_key;
-    while (from_key < top && weight(value_of(from_key)) < (double)min_p) ++from_key;
+    // mostly that key; beside a border near 0, where keys lie close, it may be many millions away: steps that double, and
+    // halves of what they leave
+    auto heavy = [&](uint32_t key) { return weight(value_of(key)) >= (double)min_p; };
+    uint32_t light = from_key, step = 1;  // in the end the key below
+    if (heavy(from_key)) {
+      for (; from_key > low_key; step *= 2) {
+        light = from_key - min(step, from_key - low_key);
+        if (!heavy(light)) break;
+        from_key = light;
+      }
+    } else {  // the largest weighs 1
+      for (;; step *= 2) {
+        from_key = light + min(step, top - light);
+        if (heavy(from_key)) break;
+        light = from_key;
+      }
+    }
+    while (from_key - light > 1) {
+      const uint32_t mid = light + (from_key - light) / 2;
+      if (heavy(mid)) from_key = mid;
+      else light = mid;
+    }
   }
   const double w_tau = tau >= from_key ? weight(value_of(tau)) : 0.0;
   const float from = value_of(max(from_key, tau + 1)), v_tau = value_of(max(tau, kNone));

@@ -632,6 +632,28 @@ def test_sample_extreme_scales():
                 check_sample(x, u, temperature=temperature, **kw)
 
 
+# largest logit, temperature, min-p (float32): the logit that weighs min-p is 0 to 10^-13 and less
+MIN_P_AT_ZERO = [(2.565428, 1.1141512, 0.1), (1.3165607, 1.0935137, 0.3), (1.9748411, 1.6402706, 0.3), (3.6204104, 1.9083719, 0.15),
+                 (3.3644526, 1.7734528, 0.15), (7.7067885, 1.9700264, 0.02), (7.156755, 1.8294256, 0.02), (4.9612117, 1.0773134, 0.01),
+                 (6.9456964, 1.5082388, 0.01), (4.117248, 1.374705, 0.05)]
+
+
+def test_sample_min_p_whose_border_is_zero():
+    """Logits one part in 10^6 to each side of such a border, where a billion
+    float32 numbers lie between it and an estimate of it."""
+    g = gen(51)
+    V = 1500
+    x = normal((len(MIN_P_AT_ZERO), V), torch.float32, g)
+    x = torch.where(x.abs() < 1e-6, torch.full_like(x, 1e-6), x).clamp(max=1.0)
+    x[:, 100], x[:, 900] = 1e-6, -1e-6
+    m, temperature, min_p = (torch.tensor(c, dtype=torch.float32, device="cuda") for c in zip(*MIN_P_AT_ZERO))
+    x[:, 700] = m
+    for u0 in (0.0, 0.3, 0.7, 1.0 - 2.0 ** -24):
+        u = torch.full_like(m, u0)
+        check_sample(x, u, temperature=temperature, min_p=min_p)
+        check_sample(x, u, temperature=temperature, min_p=min_p, top_k=1200)
+
+
 def test_sample_random_numbers_out_of_range_stay_in_the_vocabulary():
     x = normal((5, 1000), torch.float32, gen(5))
     u = torch.tensor([1.0, 2.0, -1.0, math.nan, math.inf], device="cuda")
