@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   const T* x = (const T*)p.logits + b * p.stride;
   const float temp = p.temps ? p.temps[b] : p.temp, share = p.ps ? p.ps[b] : p.p, uniform = p.u[b];
   const float min_p = p.mins ? p.mins[b] : p.min_p;
-  const int k = p.ks ? p.ks[b] : p.k;
+  const int k = min(p.ks ? p.ks[b] : p.k, V);  // from V on it cuts nothing; doubled below
   const int blk0 = me * p.per_cta;                                // first block of this CTA
   const int n_blk = max(0, min(p.per_cta, ceil_div(V, kBlock) - blk0));
   auto cluster_arrive = [&] {

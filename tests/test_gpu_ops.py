@@ -632,6 +632,19 @@ def test_sample_extreme_scales():
                 check_sample(x, u, temperature=temperature, **kw)
 
 
+@pytest.mark.parametrize("V", [40, 1500, 50001])
+def test_sample_top_k_past_the_vocabulary(V):
+    """The largest and smallest whole numbers a setting holds, as "no limit"."""
+    x = normal((10, V), torch.float32, gen(V))
+    u = torch.rand(10, generator=gen(7), device="cuda")
+    top_k = torch.tensor([V - 1, V, V + 1, 1 << 30, (1 << 30) - 1, (1 << 31) - 1, (1 << 31) - 2, -(1 << 31), -1, 0], dtype=torch.int32,
+                         device="cuda")
+    check_sample(x, u, top_k=top_k)
+    check_sample(x, u, top_k=top_k, top_p=0.9)
+    for k in ((1 << 30), (1 << 31) - 1, 1 << 40):
+        assert torch.equal(skv.sample_tokens(x, u, top_k=k), skv.sample_tokens(x, u))
+
+
 # largest logit, temperature, min-p (float32): the logit that weighs min-p is 0 to 10^-13 and less
 MIN_P_AT_ZERO = [(2.565428, 1.1141512, 0.1), (1.3165607, 1.0935137, 0.3), (1.9748411, 1.6402706, 0.3), (3.6204104, 1.9083719, 0.15),
                  (3.3644526, 1.7734528, 0.15), (7.7067885, 1.9700264, 0.02), (7.156755, 1.8294256, 0.02), (4.9612117, 1.0773134, 0.01),
