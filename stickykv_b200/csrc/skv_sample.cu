@@ -851,7 +851,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
         for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
         cluster_barrier();
       }
-      // a histogram of weights, each a whole number of 2^-14 of its bin's middle
+      // a histogram of weights, each a whole number of 2^-14 of its bin's middle, 2^-12 where a block has more than 2^17
+      // tokens (2^19 at most): all of them in one bin, each up to e^(1/60) units, stay below 2^32
+      const float units = p.per_cta * kBlock > 1 << 17 ? 4096.f : 16384.f;
       // as deep as what is further down, all V tokens of it, weighs a thousandth of what the cut leaves out
       spread(fminf(m - lowest(), temp * (logf((float)V / fmaxf(1.f - share, 1e-7f)) + 7.f)));
       const float fall = per_unit > 0.f ? 1.f / (per_unit * temp) : 0.f;  // of the weight's logarithm over a bin
@@ -862,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
         for (int i = 0; i < 8; ++i) {
           const float d = depth(v[i]), t = place(d), off = (t - 8388608.f - d) * fall;
           // e^off, |off| < 1/60 or so
-          const float part = fmaf(fmaf(off, 0.5f, 1.f), off, 1.f) * 16384.f + 8388608.f;
+          const float part = fmaf(fmaf(off, 0.5f, 1.f), off, 1.f) * units + 8388608.f;
           if (d < (float)(kBins - 2) && v[i] >= kept_from) atomicAdd(&hist[bin_at(t)], __float_as_uint(part) & 0x7fffffu);
         }
       });
@@ -876,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
         s += mass[i];
       }
       float reached = block_prefix(s) - s;
-      const float all = block_reduce(reached + s, Max()) + (tau ? (float)ties * (float)safe_weight(tau) * 16384.f : 0.f);
+      const float all = block_reduce(reached + s, Max()) + (tau ? (float)ties * (float)safe_weight(tau) * units : 0.f);
       int short_of = -1;  // the last bin that does not reach the cut
 #pragma unroll
       for (int i = 0; i < kPerThread; ++i)

@@ -700,6 +700,18 @@ def test_sample_large_vocabularies(dt, V):
         check_sample(few, u, **kw)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_sample_few_levels_of_the_largest_vocabulary(dt):
+    """Half a million tokens of a block in one bin of the weights' histogram,
+    of two levels and of one level with another beside it."""
+    V = 1 << 22
+    i = torch.arange(V, device="cuda")
+    x = torch.stack(((i % 2).float(), (i % 32 == 5).float() * 0.5, (i < V // 2).float() * 3)).to(DT[dt])
+    u = torch.rand(3, generator=gen(19), device="cuda")
+    for kw in (dict(top_p=0.3), dict(top_p=0.8), dict(top_p=0.95, temperature=0.7), dict(top_p=0.8, top_k=V - 1000), dict(top_p=0.999999)):
+        check_sample(x, u, **kw)
+
+
 def test_sample_frequencies():
     """4096 evenly spaced random numbers choose each token as often as its
     probability says, to one draw at each of its two borders."""
