@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const SampleParams 
   const int C = (int)size, me = (int)rank;
   const int b = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = p.V;
   const T* x = (const T*)p.logits + b * p.stride;
-  const float temp = p.temps ? p.temps[b] : p.temp, share = p.ps ? p.ps[b] : p.p, uniform = p.u[b];
+  const float temp = p.temps ? p.temps[b] : p.temp, uniform = p.u[b], given_share = p.ps ? p.ps[b] : p.p;
+  const float share = given_share <= 0.f ? FLT_MIN : given_share;  // one token, by way of the list as any other share
   const float min_p = p.mins ? p.mins[b] : p.min_p;
   const int k = min(p.ks ? p.ks[b] : p.k, V);  // from V on it cuts nothing; doubled below
   const int blk0 = me * p.per_cta;                                // first block of this CTA

@@ -632,6 +632,21 @@ def test_sample_extreme_scales():
                 check_sample(x, u, temperature=temperature, **kw)
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("V", [1, 700, 50001])
+def test_sample_top_p_that_keeps_one_token(V, dt):
+    """Shares of nothing and of less, with and without other cuts: the first of
+    the largest logits, thousands of them among the rows."""
+    x = normal((9, V), torch.float32, gen(V)).to(DT[dt])
+    x[1::3] = x[1::3].clamp(max=0.25)
+    x[2, V // 3] = math.inf
+    top_p = torch.tensor([0.0, 0.0, 0.0, -0.0, -1.0, -math.inf, 1e-45, 1e-38, 1e-30], device="cuda")
+    u = torch.rand(9, generator=gen(7), device="cuda")
+    for kw in (dict(), dict(top_k=5), dict(top_k=600), dict(temperature=100.0), dict(temperature=1e-30), dict(min_p=0.5)):
+        got = check_sample(x, u, top_p=top_p, **kw)
+        assert got.tolist() == np.argmax(x.float().cpu().numpy(), 1).tolist()
+
+
 @pytest.mark.parametrize("V", [40, 1500, 50001])
 def test_sample_top_k_past_the_vocabulary(V):
     """The largest and smallest whole numbers a setting holds, as "no limit"."""
