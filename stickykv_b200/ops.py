@@ -17,6 +17,7 @@ from typing import Any, Dict, Optional, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from ._lib import RotaryArgs, SampleArgs, WindowArgs, check, lib
 from .cache import _DT, _cur_dev, _on, _raw_stream, _stream
@@ -44,8 +45,9 @@ def _meta(t: Optional[Tensor]) -> Optional[tuple]:
 
 def _ready(index: int, *tensors: Optional[Tensor]) -> bool:
     """All on GPU ``index``, which is the current one, and none asks for
-    gradients: nothing is left to check but the plan's key."""
-    if index < 0 or _cur_dev is None or _raw_stream is None or _cur_dev() != index:
+    gradients (none can carry a tangent outside of forward-mode levels): nothing
+    is left to check but the plan's key."""
+    if index < 0 or _cur_dev is None or _raw_stream is None or _cur_dev() != index or forward_ad._current_level >= 0:
         return False
     grad = torch.is_grad_enabled()
     for t in tensors:
@@ -68,6 +70,8 @@ def _cuda(what: str, device: torch.device) -> None:
 def _no_grad(what: str, *tensors: Optional[Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError(f"{what} has no backward pass: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no derivative: call it on tensors without tangents")
 
 
 def _setting(what: str, x: Any, kind: type) -> Any:

@@ -463,6 +463,19 @@ def test_settings_in_tensors_are_read_at_each_call(device):
     assert torch.equal(skv.sample_tokens(x, u, top_k=top_k), skv.sample_tokens(x, u, top_k=4))
 
 
+def test_tangents_are_refused_of_repeated_calls():
+    from torch.autograd import forward_ad
+    q, k, v = qkv(2, 1, 64, 4, 2, 64, "f16", 1)
+    want = [skv.sink_window_attention(q, k, v, window=9) for _ in range(2)][0]
+    with forward_ad.dual_level():
+        assert torch.equal(skv.sink_window_attention(q, k, v, window=9), want)
+        for i in range(3):
+            x = [q, k, v]
+            x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises(NotImplementedError, match="no derivative"):
+                skv.sink_window_attention(*x, window=9)
+
+
 def test_window_past_32_bit_offsets():
     """A cache of over 2^31 elements, most of it never written; decode and a
     chunk at its far end and, with sinks, at its beginning."""

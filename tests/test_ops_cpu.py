@@ -142,6 +142,22 @@ def test_settings_are_numbers(call, kw, error):
         call(**kw)
 
 
+@pytest.mark.parametrize("call, name, x", [
+    (_rotary, "query", torch.zeros(2, 4, 3, 16)), (_rotary, "key", torch.zeros(2, 2, 3, 16)), (_rotary, "inv_freq", torch.ones(8)),
+    (_window, "query", torch.zeros(2, 4, 3, 16)), (_window, "value", torch.zeros(2, 2, 9, 16)), (_window, "scaling", torch.tensor(0.5)),
+    (_sample, "logits", torch.zeros(2, 5)), (_sample, "temperature", torch.ones(2)), (_sample, "uniform", torch.zeros(2)),
+])
+def test_tangents_are_refused(call, name, x):
+    """Forward-mode derivatives, which would be dropped."""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="no derivative"):
+        call(**{name: forward_ad.make_dual(x, torch.ones_like(x))})
+    with pytest.raises(NotImplementedError, match="no derivative"):
+        torch.func.jvp(lambda y: call(**{name: y}), (x,), (torch.ones_like(x),))
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no CPU path"):
+        call()
+
+
 # -- C entries: every refusal comes before anything is launched ---------------------------
 
 _P = 1 << 20  # an aligned address that nothing reads
