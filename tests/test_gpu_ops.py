@@ -695,6 +695,24 @@ def test_sample_min_p_whose_border_is_zero():
         check_sample(x, u, temperature=temperature, min_p=min_p, top_k=1200)
 
 
+def test_sample_weights_are_64_bit():
+    """Logits whose weights differ from min-p by 4e-15 of it and more, to either
+    side: as many times what 64-bit roundings move (an exponent of 4 and an
+    exponential, together under 1e-15).  The last kept token is drawn."""
+    rows = []
+    for m, temperature, min_p in MIN_P_AT_ZERO:
+        at = np.longdouble(np.float32(m)) + np.log(np.longdouble(np.float32(min_p))) * np.longdouble(np.float32(temperature))
+        for near in (0.0, at - 1e-14, at + 1e-14, at - 1e-13, at + 1e-13, at - 1e-12, at + 1e-12):
+            if abs(np.longdouble(np.float32(near)) - at) > 4e-15 * temperature:
+                rows.append((m, float(np.float32(near)), -20.0, temperature, min_p))
+    assert len(rows) > 55
+    t = torch.tensor(rows, dtype=torch.float32, device="cuda")
+    u = torch.full((len(rows),), 1.0 - 2.0 ** -24, device="cuda")
+    x, temperature, min_p = t[:, :3].contiguous(), t[:, 3].contiguous(), t[:, 4].contiguous()
+    got = check_sample(x, u, temperature=temperature, min_p=min_p)
+    assert set(got.tolist()) == {0, 1}
+
+
 def test_sample_random_numbers_out_of_range_stay_in_the_vocabulary():
     x = normal((5, 1000), torch.float32, gen(5))
     u = torch.tensor([1.0, 2.0, -1.0, math.nan, math.inf], device="cuda")
