@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t sQ = base, sR = base + 2 * C::kTile, bars = sR + C::kStages * C::kTile;
   const uint32_t bQ = bars, bFull = bars + 8, bFree = bFull + 8 * C::kStages, bS = bFree + 8 * C::kStages,
-                 bL = bS + 16, bP = bL + 16, bP2 = bP + 16, bO = bP2 + 16, sAddr = bO + 16;
+                 bL = bS + 16, bP = bL + 16, bP2 = bP + 16, bO = bP2 + 16, sAddr = bO + 16, sLost = sAddr + 4;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kh = blockIdx.y, b = blockIdx.z;
   const int G = p.Hq / p.Hkv, TQ = kRows / G;                // tokens of a tile
@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
   if (warp == 9 && lane == 0) {
+    asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(sLost), "r"(0u) : "memory");
     bar_init(bQ, 1);
     for (int s = 0; s < 2 * C::kStages; ++s) bar_init(bFull + 8 * s, 1);
     for (int t = 0; t < 2; ++t) {
@@ -149,19 +150,34 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(tmem) : "r"(sAddr));
-  bool lost = false;  // a wait ran out: the rest is not waited for, and the rows are done again key by key
+  // a wait ran out: the rest is not waited for, and the rows are done again key by key; all rows of the block where it was
+  // one of warps 8 or 9, which say so in sLost
+  bool lost = false;
+  auto say_lost = [&] { asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(sLost), "r"(1u) : "memory"); };
+  auto meet = [&] {  // the block's end, from either side of the branch
+    fence_before();
+    asm volatile("bar.sync 1, %0;\n" ::"n"(kThreads) : "memory");
+    fence_after();
+  };
 
   // 168 registers a thread at launch, three warpgroups: 2 x 208 + 80 of the 504 they share
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n" ::);
     if (warp == 9) {
-      if (lane == 0) {
-        for (int x = 1; x < 2 * n; ++x) {
+      if (lane == 0 && n > 0) {
+        int x = 1;
+        for (; x < 2 * n; ++x) {
           const int s = x % C::kStages, use = x / C::kStages;
           if (use > 0 && !bar_wait(bFree + 8 * s, (use - 1) & 1)) break;
           load_kv(x);
         }
+        lost = x < 2 * n;
+        // no copy outlives the block, even where warp 8 waits no more: the last one into each place of the ring
+        lost |= !bar_wait(bQ, 0);
+        for (int y = max(0, x - C::kStages); y < x; ++y) lost |= !bar_wait(bFull + 8 * (y % C::kStages), (y / C::kStages) & 1);
+        if (lost) say_lost();
       }
+      __syncwarp();
     } else if (warp == 8) {
       if (n > 0) {
         auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -226,9 +242,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             commit(bFree + 8 * ((2 * j + 2) % C::kStages));
           }
         }
+        if (lost) say_lost();
       }
       __syncwarp();
     }
+    meet();
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n" ::);
     const int t = warp >> 2, rl = threadIdx.x & 127;
@@ -371,18 +390,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // a key that is not finite reaches the rows that do not see it as 0 * inf:
     // rows that come out not finite are done again key by key
-    __syncwarp();  // behind the stores above
-    uint32_t again = __ballot_sync(0xffffffffu, bad && real);
+    meet();  // behind the stores above
+    uint32_t all;
+    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(all) : "r"(sLost) : "memory");
+    uint32_t again = __ballot_sync(0xffffffffu, (bad || all) && real);
     while (again) {
       const int who = __ffs(again) - 1;
       again &= again - 1;
       window_one_row<T, D>(p, row, b, __shfl_sync(0xffffffffu, h, who), __shfl_sync(0xffffffffu, token, who), lane, 0, D);
     }
   }
-  fence_before();
-  __syncthreads();
-  fence_after();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
 }
 
 template <typename T, int D>
