@@ -4,7 +4,9 @@
 // contexts reach 10^6 and more, where a 32-bit product is off by a tenth of a
 // radian; the product is taken in 64 bits, in turns (a / 2 pi), reduced to
 // half a turn to each side there, and only the rest goes to a 32-bit sine and
-// cosine.
+// cosine.  For float32 the part of the angle that 32 bits leave out is added to
+// both (without it results were off by 5.6e-8 of their size, root mean square;
+// products in 64 bits rounded once 4.2e-8); 16-bit results do not show it.
 //
 // A block owns 32 chunks of 2V channels, of one token or several, for four
 // heads at a time: it takes the sines and cosines of its chunks once, through
@@ -117,8 +119,14 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) 
     if (k < p.rot_chunks) {
       double turn = where[i / V] * (double)p.inv_freq[V * k + i % V];
       turn -= (turn + 6755399441055744.0) - 6755399441055744.0;  // 1.5 * 2^52: rounds to whole turns
+      const float a = (float)(2.0 * turn);
       float s, co;
-      sincospif((float)(2.0 * turn), &s, &co);
+      sincospif(a, &s, &co);
+      if constexpr (sizeof(T) == 4) {  // and what the angle's rounding left over, up to 2^-25, to first order
+        const float left = (float)(2.0 * turn - (double)a) * 3.14159265f, s0 = s;
+        s = fmaf(co, left, s);
+        co = fmaf(-s0, left, co);
+      }
       turns[i] = make_float2(co * p.scale, s * p.scale * p.sgn);
     }
   }

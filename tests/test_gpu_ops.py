@@ -86,6 +86,28 @@ def test_rotary(B, T, Hq, Hkv, D, r, inter, dt):
             assert torch.equal(y[..., r:], x[..., r:])
 
 
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotary_float32_counts_the_whole_angle(inter, inverse):
+    """Each term of a result is off by what it is made of, small cosines and
+    sines included: 2 * 2^-24 of sincospi (1 ulp), a rounding of the rest of the
+    angle's share, of the product and of the sum, 6 in all with the result's
+    own; the angle by four roundings of 64 bits and 2^-46."""
+    g = gen(21)
+    B, H, T, D = 2, 3, 700, 64
+    x = normal((B, H, T, D), torch.float32, g)
+    pos = torch.randint(0, 1 << 20, (B, T), generator=g, device="cuda")
+    inv, _ = skv.rotary_frequencies(D, 500000.0, device="cuda")
+    a = pos.double()[:, None, :, None] * inv.double() * (-1 if inverse else 1)
+    c, s, e = a.cos(), a.sin(), a.abs() * 4 * 2.0 ** -53 + 2.0 ** -46
+    i = torch.arange(D, device="cuda")
+    i0, i1 = (i[0::2], i[1::2]) if inter else (i[:D // 2], i[D // 2:])
+    x0, x1 = x[..., i0].double(), x[..., i1].double()
+    got, _ = skv.apply_rotary(x, None, pos, inv, interleaved=inter, inverse=inverse)
+    for j, p, q, name in ((i0, x0 * c, -x1 * s, "first"), (i1, x1 * c, x0 * s, "second")):
+        within(got[..., j], p + q, 6 * U32 * (p.abs() + q.abs()) + e * (x0.abs() + x1.abs()), name)
+
+
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("inter", [False, True])
 def test_rotary_in_place_on_slices_of_one_projection(dt, inter):
