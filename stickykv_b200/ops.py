@@ -85,14 +85,16 @@ def _setting(what: str, x: Any, kind: type) -> Any:
 
 
 def _overlap(a: Tensor, b: Tensor) -> bool:
-    """Whether two tensors without gaps meet in memory.  Tensors with gaps
-    (slices of one projection's output, whose rows alternate) are the
-    caller's to keep apart."""
+    """Whether two tensors without gaps meet in memory, or two of any kind begin
+    at one address.  Others with gaps (slices of one projection's output, whose
+    rows alternate) are the caller's to keep apart."""
     def span(t: Tensor) -> Tuple[int, int, bool]:
         n = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
         return t.data_ptr(), t.data_ptr() + n * t.element_size(), n == t.numel()
     if not a.numel() or not b.numel():
         return False
+    if a.data_ptr() == b.data_ptr():
+        return True
     (a0, a1, whole_a), (b0, b1, whole_b) = span(a), span(b)
     return whole_a and whole_b and a0 < b1 and b0 < a1
 

@@ -235,6 +235,21 @@ def test_window(B, T, S, Hq, Hkv, window, sinks, dt, D):
     check_window(q, k, v, window, sinks)
 
 
+@pytest.mark.parametrize("B, T, S, Hq, Hkv, window, sinks", WINDOW)
+def test_window_bf16_heads_of_16(B, T, S, Hq, Hkv, window, sinks):
+    q, k, v = qkv(B, T, S, Hq, Hkv, 16, "bf16", 7 * T + S)
+    check_window(q, k, v, window, sinks)
+
+
+@pytest.mark.parametrize("dt, D, B, T, window", [("bf16", 64, 4, 900, 200), ("f16", 128, 2, 1111, 500), ("f16", 64, 16, 1, 900),
+                                                 ("f32", 64, 3, 130, 100), ("bf16", 16, 2, 300, 77)])
+def test_window_equal_calls_give_equal_bits(dt, D, B, T, window):
+    q, k, v = qkv(B, T, 1200, 32, 8, D, dt, 6)
+    want = skv.sink_window_attention(q, k, v, window=window, sinks=4)
+    for _ in range(4):
+        assert torch.equal(skv.sink_window_attention(q, k, v, window=window, sinks=4), want)
+
+
 @pytest.mark.parametrize("dt, D", [("f16", 64), ("bf16", 64), ("f16", 128), ("bf16", 128)])
 @pytest.mark.parametrize("T, S, Hq, Hkv", [(64, 64, 4, 4), (100, 100, 8, 2), (127, 127, 4, 1), (128, 128, 4, 2), (129, 257, 8, 2),
                                            (260, 260, 3, 3), (300, 1111, 8, 2), (90, 90, 100, 1), (33, 33, 128, 1)])

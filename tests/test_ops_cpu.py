@@ -57,6 +57,21 @@ def test_rotary_refuses_outputs_that_overlap():
         _rotary(query=q, key=k, out=(q, k))
 
 
+def test_outputs_that_begin_where_another_tensor_does_are_refused():
+    """Slices with gaps: an output over the other input, over its own input in
+    another order, and both outputs in one place."""
+    buf = torch.zeros(2, 3, 8, 16)
+    q, k = buf[:, :, :2].transpose(1, 2), buf[:, :, 2:4].transpose(1, 2)
+    for out in ((k, q), (q, q), (buf.view(2, 4, 6, 16)[:, :2, :3], k)):
+        with pytest.raises(ValueError, match="overlap"):
+            _rotary(query=q, key=k, out=out)
+    with pytest.raises(ValueError, match="overlaps"):
+        _window(query=buf[:1, :, :4].transpose(1, 2), key=torch.zeros(1, 2, 9, 16), value=torch.zeros(1, 2, 9, 16),
+                out=buf.view(-1)[:3 * 4 * 16].view(1, 3, 4, 16))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        _rotary(query=q, key=k, out=(q, k))
+
+
 def _window(**kw):
     a = dict(query=torch.zeros(2, 4, 3, 16), key=torch.zeros(2, 2, 9, 16), value=torch.zeros(2, 2, 9, 16), window=4)
     a.update(kw)
