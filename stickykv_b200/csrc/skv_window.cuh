@@ -1,6 +1,8 @@
 // Parameters and row bounds shared by the window-attention kernels.
 #pragma once
 
+#include <type_traits>
+
 #include "skv_common.cuh"
 
 namespace skv {
@@ -33,5 +35,10 @@ __device__ __forceinline__ WindowRow window_row(const WindowParams& p, int b) {
   r.first = p.slots ? min(max(p.slots[b], -(1 << 30)), p.S) : r.end - p.T;
   return r;
 }
+
+// Weights 2^(score - m) go to fp16 times 2^7: up to 2^15 (m lags by 2^8 at
+// most), and the subnormals, whose step is a constant, begin at 2^-21 of the
+// largest in place of 2^-14.  The factor cancels in the quotient.
+template <typename T> __device__ constexpr float weight_lift() { return std::is_same<T, __half>::value ? 7.f : 0.f; }
 
 }  // namespace skv

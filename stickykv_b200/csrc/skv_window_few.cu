@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(FewCfg<T, D, NT>::kWarps * 32, FewCfg<T, D, NT
       float w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        w[e] = s[n][e] == -INFINITY ? 0.f : ex2(s[n][e] - m[n][e & 1]);
+        w[e] = s[n][e] == -INFINITY ? 0.f : ex2(s[n][e] - m[n][e & 1] + weight_lift<T>());
         l[n][e & 1] += w[e];
       }
 #pragma unroll

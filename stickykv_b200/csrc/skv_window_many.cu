@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float mm = m == -INFINITY ? 0.f : m;
       // P = exp2(S - m), two of the multiply-adds an instruction (scalar ones: 7 % slower)
-      const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(-mm, -mm);
+      const float2 scale2 = make_float2(sl2, sl2), shift2 = make_float2(weight_lift<T>() - mm, weight_lift<T>() - mm);
       float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       auto weigh = [&](int i) {
         float2 x = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), scale2, shift2);

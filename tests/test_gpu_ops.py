@@ -398,6 +398,27 @@ def test_window_whole_shares_of_scores_that_are_nan(dt, D, lo, hi):
     assert got[:, :, 2:].isnan().all() and torch.equal(got[:, :, :2], want[:, :, :2])
 
 
+@pytest.mark.parametrize("dt, D", [("f16", 16), ("f16", 64), ("f16", 128), ("bf16", 64), ("f32", 32)])
+@pytest.mark.parametrize("T, rows", [(1, 1), (1, 40), (9, 2), (333, 60)])
+def test_window_weights_far_below_the_largest(dt, D, T, rows):
+    """A first token that takes nearly all weight and holds zeros: the output is
+    made of weights from 2^-12 to 2^-25 of the largest.  fp16 weights are scaled
+    to at most 2^15, the largest to 2^7 at least, so below 2^-14 they are off by
+    2^-25 / 2^7 of it at most (two terms: less), on top of the usual bound."""
+    S, window = 333, 170
+    q, k, v = qkv(rows, T, S, 4, 2, D, dt, 17)
+    q.zero_()
+    q[..., 0] = 1
+    k[..., 0] = -8.5 - 8.5 * torch.rand(rows, 2, S, generator=gen(18), device="cuda")
+    k[:, :, 0, 0] = 0
+    v.mul_(64)
+    v[:, :, 0] = 0
+    got = skv.sink_window_attention(q, k, v, window=window, sinks=1, scaling=1.0)
+    ref = window_ref(q, k, v, window, 1, scaling=1.0)
+    size = window_ref(torch.zeros_like(q), k, v, window, 1)  # of equal weights: A is the mean of |v|
+    within(got, ref[0], window_tol(q, ref) + (2.0 ** -32 * size[1] * size[3] if dt == "f16" else 0.0))
+
+
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("B, T", [(2, 1), (2, 40), (60, 150)])
 def test_window_strides(dt, B, T):
