@@ -341,7 +341,8 @@ int skv_window_attention(const skv_window_args* args, void* stream);
 
 /*
  * Next token of each row.  With x the row's logits (NaN counts as -inf), m
- * its largest and w_i = exp((x_i - m) / temperature) in 64 bits, tokens in
+ * its largest and w_i = exp((x_i - m) / temperature) in 64 bits (right to a
+ * rounding or two; beside a cut to 2^-52 of the largest), tokens in
  * descending order of x (equal ones by ascending index):
  *   top_k > 0   keeps the first top_k;
  *   top_p < 1   keeps of those the fewest first ones whose mass reaches

@@ -5,8 +5,9 @@
 // radian; the product is taken in 64 bits, in turns (a / 2 pi), reduced to
 // half a turn to each side there, and only the rest goes to a 32-bit sine and
 // cosine.  For float32 the part of the angle that 32 bits leave out is added to
-// both (without it results were off by 5.6e-8 of their size, root mean square;
-// products in 64 bits rounded once 4.2e-8); 16-bit results do not show it.
+// both (results are off by 4.1e-8 of their size, root mean square, without it by
+// 5.6e-8; 204 us with and without for the tensors below); 16-bit results do not
+// show it.
 //
 // A block owns 32 chunks of 2V channels, of one token or several, for four
 // heads at a time: it takes the sines and cosines of its chunks once, through

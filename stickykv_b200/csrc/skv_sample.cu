@@ -3,9 +3,10 @@
 //
 // In descending order with ties by index every cut is a threshold: the key of
 // the last kept token and how many of its equals, lowest indices first, stay.
-// No sort.  A cluster holds a row in its blocks' shared memory; every 256
-// tokens' largest is kept beside them, and passes skip those below what they
-// look for.
+// No sort.  A cluster holds a row in its blocks' shared memory (up to 315
+// thousand float32 or 630 thousand 16-bit tokens; of a longer row every pass
+// reads global memory); every 256 tokens' largest is kept beside them, and
+// passes skip those below what they look for.
 //   few of top-k   a value that k of those maxima reach bounds the cut; the
 //                  tokens from there on, little more than k, are listed;
 //   top-k, top-p   a histogram (counts, weights) over evenly spaced values
@@ -17,14 +18,18 @@
 //
 // Weights and sums are 64-bit: a draw falls between two neighbours of 10^5
 // cumulative sums, and 32-bit sums would move a share of draws to a neighbour.
-// Sums are taken in a fixed order, or as whole numbers where the order is not
-// fixed, so equal calls give equal tokens.
+// Sums are taken in a fixed order, or, where the order is not fixed, as whole
+// numbers of 2^-52 of the largest weight (the step of a 64-bit sum of which that
+// is part), so equal calls give equal tokens.
 //
 // Bound: one row is latency, three to six cluster barriers (32000 tokens: greedy
-// 2.9 us, top-k 50 12 us, with top-p 0.95 14 us); many rows the 64-bit
-// exponentials of a top-p cut, 13 operations a token at 59 a clock and SM, twice
-// (128 rows x 128256 bf16: greedy 12 us, 2.8 TB/s; temperature 43 us; top-p 0.9
-// 116 us).  HBM is read once.
+// 3.3 us, top-k 50 13 us, with top-p 0.95 15 us).  Many rows: rounds of blocks,
+// one an SM (16 warps; shared memory and registers hold no second), whose warps
+// wait for their own last results with nobody to step in: issue at 51 %, the
+// 64-bit pipe at 24 %, HBM read once (rows that fit).  128 rows x 128256 bf16 are
+// two rounds: greedy 12 us, 2.8 TB/s; temperature 46 us; top-p 0.9 119 to 125 us
+// (74 rows, one round: 6.6, 24, 65 us).  A block of 256 tokens of which one is
+// kept is weighed whole, at a top-p cut twice.
 #include <float.h>
 
 #include <type_traits>
@@ -1132,7 +1137,7 @@ int launch(SampleParams p, int batch, cudaStream_t stream) {
   constexpr int kMost = 160 * 1024;  // bytes of a row's share in shared memory, beside 36 KB of histogram and list
   const int blocks = ceil_div(p.V, kBlock);
   // a cluster at least as large as holds the row, and as large as keeps every
-  // warp busy with all rows resident (a block an SM, of 114 registers a thread:
+  // warp busy with all rows resident (a block an SM, of 124 registers a thread:
   // 33 rows on clusters of 8, two rounds, took twice as long as on 4)
   int c = 1;
   auto bytes = [&](int n) {

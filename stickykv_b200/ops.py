@@ -353,8 +353,10 @@ def sink_window_attention(query: Tensor, key: Tensor, value: Tensor, *, window: 
     token).  So a left-padded prompt gives ``starts``, a right-padded one
     ``ends`` and zero ``query_slots``, a decode step over a preallocated cache
     ``ends``.  A query that sees no key (padding), or only scores of -inf,
-    gets zeros; what a query does not see never reaches its output, whatever
-    it holds."""
+    gets zeros, one with a NaN or +inf among its scores NaN; what a query does
+    not see never reaches its output, whatever it holds.  Sums are in 32 bits;
+    prompts and chunks of 16-bit types may round the weights to their type
+    before the product with ``value``."""
     if window.__class__ is not int or sinks.__class__ is not int or scaling is not None:
         window, sinks = _setting("sink_window_attention", window, int), _setting("sink_window_attention", sinks, int)
         scaling = _setting("sink_window_attention", scaling, float)
@@ -443,7 +445,8 @@ def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Union[float, 
     ``top_p < 1`` the fewest first ones of those whose mass reaches top_p of
     theirs, ``min_p`` those of at least min_p times the largest weight.  The
     token is the first, in the vocabulary's order, at which the cumulative
-    kept mass exceeds ``uniform`` times the kept mass; sums are in 64 bits.
+    kept mass exceeds ``uniform`` times the kept mass.  Weights and sums are in
+    64 bits (a top-p cut takes weights to 2^-52 of the largest).
 
     ``temperature`` 0 takes the largest logit (the lowest index of equal
     ones).  NaN logits count as -inf; a row with nothing above -inf gives -1.
