@@ -91,7 +91,9 @@ __device__ __forceinline__ void window_join(const WindowParams& p, const WindowR
       }
     }
     const float res = sum == 0.f ? 0.f : val / sum;
-    repair |= !(fabsf(res) < INFINITY);
+    // (a sum of NaN is a NaN or +inf among the row's own scores, and NaN its answer; in float32 also an infinite channel,
+    // whose two terms make a NaN of any score)
+    repair |= !(fabsf(res) < INFINITY) && (sum == sum || std::is_same<T, float>::value);
     const int rr = r0 + r;
     st_f32((T*)p.out + (((int64_t)b * p.T + rr / G) * p.Hq + kh * G + rr % G) * D + d, res);
   }

@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         const float y = l == 0.f ? 0.f : __uint_as_float(x[i]) * inv;
-        bad |= !(fabsf(y) < INFINITY);
+        bad |= !(fabsf(y) < INFINITY) && l == l;
         x[i] = __float_as_uint(y);
       }
       if (real) {
@@ -396,7 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     // a key that is not finite reaches the rows that do not see it as 0 * inf:
-    // rows that come out not finite are done again key by key
+    // rows that come out not finite are done again key by key (but for those whose own scores hold a NaN or +inf, l's
+    // only way to be NaN)
     meet();  // behind the stores above
     uint32_t all;
     asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(all) : "r"(sLost) : "memory");

@@ -534,6 +534,33 @@ def test_tangents_are_refused_of_repeated_calls():
                 skv.sink_window_attention(*x, window=9)
 
 
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("T, D", [(1, 64), (30, 32), (700, 64), (700, 128)])
+def test_window_of_nan_queries_takes_no_longer(T, D, dt):
+    """Rows whose own scores are NaN are not done again key by key, which takes
+    from 30 to 500 times as long: a call of nothing but NaN stays within five
+    times the call of finite numbers (the same work, timed by the fastest of
+    several)."""
+    q, k, v = qkv(8, T, 4000, 32, 8, D, dt, 23)
+    bad = torch.full_like(q, math.nan)
+
+    def fastest(x):
+        times = []
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda._sleep(100000)
+            a.record()
+            out = skv.sink_window_attention(x, k, v, window=2000, sinks=4)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times), out
+
+    finite, _ = fastest(q)
+    nan, out = fastest(bad)
+    assert out.isnan().all() and nan < 5 * finite
+
+
 def test_window_past_32_bit_offsets():
     """A cache of over 2^31 elements, most of it never written; decode and a
     chunk at its far end and, with sinks, at its beginning."""
