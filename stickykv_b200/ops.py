@@ -134,7 +134,7 @@ def rotary_frequencies(rotary_dim: int, theta: Optional[float] = None, scaling: 
       1``, or ``g(mscale) / g(mscale_all_dim)`` where both are given and not 0."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be a positive even number, got {rotary_dim}")
-    cfg = {name: v for name, v in (scaling or {}).items() if v is not None}
+    cfg = {name: v for name, v in (scaling or {}).items() if v is not None or name == "truncate"}
     kind = cfg.get("rope_type", cfg.get("type", "default"))
     unknown = sorted(str(name) for name in cfg if name not in _ROPE_KEYS)
     if unknown:
@@ -191,6 +191,7 @@ def rotary_frequencies(rotary_dim: int, theta: Optional[float] = None, scaling: 
         lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
         ramp = ((i / 2 - lo) / (hi - lo if hi != lo else 0.001)).clamp(0.0, 1.0)
         freq = freq * ((1.0 - ramp) + ramp / factor)
+
         def growth(m: float) -> float:
             return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
 

@@ -307,7 +307,7 @@ _YARN = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings"
     dict(_YARN, mscale=1.0, mscale_all_dim=0.707), dict(_YARN, mscale=0.707), dict(_YARN, mscale_all_dim=0.707),
     dict(_YARN, mscale=0.0, mscale_all_dim=1.0), dict(_YARN, mscale=1.0, mscale_all_dim=0.707, attention_factor=1.1),
     dict(_YARN, factor=1.0, mscale=0.5, mscale_all_dim=1.0), dict(_YARN, attention_factor=None, mscale=2.0, mscale_all_dim=0.5),
-    dict(_YARN, beta_fast=16.0, truncate=False), {"rope_type": "default"},
+    dict(_YARN, beta_fast=16.0, truncate=False), dict(_YARN, truncate=None), dict(_YARN, beta_fast=None), {"rope_type": "default"},
     {"rope_type": "linear", "factor": 4.0, "original_max_position_embeddings": 512},
 ])
 def test_frequencies_of_whole_dicts_are_those_of_transformers(scaling):
